@@ -32,10 +32,15 @@ BOA_WEIGHTS_F16 = 2
 BOA_WEIGHTS_TF32X3 = 3
 BOA_WEIGHTS_F16X2 = 4
 
+BOA_DTYPE_F32 = 0
+BOA_DTYPE_BF16 = 1
+BOA_DTYPE_F16 = 2
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
+_F = ctypes.c_float
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -67,6 +72,18 @@ SIGNATURES = {
     "boa_diag_gemm": [_I, _I, _I, _P, _P, _P, _I],
     "boa_model_step": [_P, _I, _P, _P, _P, _SZ, _P],
     "boa_model_logits": [_P, _I, _I, _P, _P, _P, _SZ, _P],
+    "boa_layer_norm": [_I64, _I, _I, _P, _I64, _P, _P, _F, _P, _P, _I, _P],
+    "boa_layer_norm_workspace_bytes": [_I64, _I, _I],
+    "boa_layer_norm_backward": [_I64, _I, _I, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _SZ, _I, _P],
+    "boa_causal_conv": [_P, _P],
+    "boa_causal_conv_workspace_bytes": [_P],
+    "boa_causal_conv_backward": [_P, _P],
+    "boa_causal_conv_step": [_P, _P],
+    "boa_ssm_checkpoint_bytes": [_P],
+    "boa_ssm_workspace_bytes": [_P, _I],
+    "boa_ssm_scan": [_P, _P],
+    "boa_ssm_scan_backward": [_P, _P],
+    "boa_ssm_step": [_P, _P],
     "boa_codec_encode": [_P, _I, _P, _I64, _P, _P, _I, _P, _I, _P, _SZ, _P],
     "boa_codec_decode": [_P, _I, _P, _I, _P, _P, _P, _P, _I64, _I, _P, _SZ, _P],
     "boa_codec_encode_range": [_P, _I, _P, _I64, _P, _I, _I, _P, _I, _P, _I, _P, _SZ, _P],
@@ -75,7 +92,36 @@ SIGNATURES = {
 _RESTYPES = {
     "boa_last_error": ctypes.c_char_p,
     "boa_model_workspace_bytes": ctypes.c_size_t,
+    "boa_layer_norm_workspace_bytes": ctypes.c_size_t,
+    "boa_causal_conv_workspace_bytes": ctypes.c_size_t,
+    "boa_ssm_checkpoint_bytes": ctypes.c_size_t,
+    "boa_ssm_workspace_bytes": ctypes.c_size_t,
 }
+
+
+class ConvArgs(ctypes.Structure):
+    """boa_conv_args."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "batch", "length", "channels", "width", "silu", "device",
+                                               "reserved")]
+                + [("x", _P), ("x_bs", _I64), ("x_ts", _I64)]
+                + [(n, _P) for n in ("weight", "bias", "state", "lens", "y", "state_out", "dy")]
+                + [("dy_bs", _I64), ("dy_ts", _I64)]
+                + [(n, _P) for n in ("dstate_out", "dx", "dweight", "dbias", "dstate", "workspace")]
+                + [("workspace_bytes", _SZ)])
+
+
+class SsmArgs(ctypes.Structure):
+    """boa_ssm_args."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "batch", "length", "channels", "states", "softplus", "device",
+                                               "reserved")]
+                + [(n, _P) for n in ("x", "dt", "z", "B", "C")]
+                + [(n, _I64) for n in ("x_bs", "x_ts", "dt_bs", "dt_ts", "z_bs", "z_ts", "B_bs", "B_ts", "C_bs",
+                                       "C_ts")]
+                + [(n, _P) for n in ("A", "D", "dt_bias", "state", "lens", "y", "state_out", "checkpoints", "dy")]
+                + [("dy_bs", _I64), ("dy_ts", _I64)]
+                + [(n, _P) for n in ("dstate_out", "dx", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dstate",
+                                     "workspace")]
+                + [("workspace_bytes", _SZ)])
 
 _lib = None
 _lock = threading.Lock()

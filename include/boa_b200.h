@@ -246,6 +246,128 @@ BOA_API int boa_codec_decode_range(boa_model* m, int n_chunks, const uint32_t* d
                                    void* d_workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Operators of a Mamba block outside its matrix products (model.py:42-65    */
+/* and the mixer that model.py:47 takes from a library): layer norm, the     */
+/* causal depthwise convolution and the selective state space scan, over     */
+/* whole sequences with their gradients and for one token per stream.        */
+/* Activations are fp32, bf16 or fp16 (one type per call); parameters,       */
+/* statistics, scan states and parameter gradients are fp32.  Sequences are  */
+/* [batch, length, channels] with channels contiguous; *_bs and *_ts are the */
+/* batch and token strides in elements, so slices of wider rows need no      */
+/* copy.  Outputs are contiguous.  Every call only enqueues work on `stream` */
+/* and runs on device `device`; nothing is kept between calls.  Sums have a  */
+/* fixed order: equal inputs give equal bits on equal devices, but a row's   */
+/* last bits may depend on the sizes of the call (the scan's split of the    */
+/* length follows them).                                                     */
+/* ------------------------------------------------------------------------ */
+#define BOA_DTYPE_F32 0
+#define BOA_DTYPE_BF16 1
+#define BOA_DTYPE_F16 2
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis
+ * (nn.LayerNorm, model.py:45,51).  x is [rows, width] with row stride x_stride;
+ * y is contiguous; bias may be NULL.  stats (NULL, or 2 * rows floats) receives
+ * mean and 1/sqrt(var + eps) of every row for the backward call.  width is in
+ * [1, 8192] (BOA_ERR_UNSUPPORTED beyond). */
+BOA_API int boa_layer_norm(int64_t rows, int width, int dtype, const void* d_x, int64_t x_stride,
+                           const float* d_weight, const float* d_bias, float eps, void* d_y, float* d_stats,
+                           int device, void* stream);
+/* Bytes of workspace for boa_layer_norm_backward (0 on a bad argument). */
+BOA_API size_t boa_layer_norm_workspace_bytes(int64_t rows, int width, int dtype);
+/* Gradients from dy: dx (contiguous), dweight, dbias (may be NULL). */
+BOA_API int boa_layer_norm_backward(int64_t rows, int width, int dtype, const void* d_x, int64_t x_stride,
+                                    const void* d_dy, int64_t dy_stride, const float* d_weight,
+                                    const float* d_stats, void* d_dx, float* d_dweight, float* d_dbias,
+                                    void* d_workspace, size_t workspace_bytes, int device, void* stream);
+
+/* Causal depthwise convolution of width 2..4 with optional SiLU:
+ *   p_t = bias + sum_k weight[:, k] * x_{t - width + 1 + k},  y = silu(p) or p.
+ * `state` [batch, width - 1, channels] (NULL: zeros) holds the inputs before
+ * position 0, oldest first; state_out (may be NULL) receives the last
+ * width - 1 inputs of every row.  lens [batch] (int32, NULL: length) gives each
+ * row's valid length, clamped to [0, length]; positions behind it are not read
+ * and their y and dx are zero.  The fields behind `state_out` are the backward
+ * call's: dy, dstate_out (NULL: zeros) in; dx, dweight, dbias (NULL when bias
+ * is), dstate (may be NULL) out. */
+typedef struct boa_conv_args {
+  int32_t dtype, batch, length, channels, width, silu, device, reserved;
+  const void* x;
+  int64_t x_bs, x_ts;
+  const float* weight; /* [channels, width] */
+  const float* bias;   /* [channels] or NULL */
+  const void* state;
+  const int32_t* lens;
+  void* y;
+  void* state_out;
+  const void* dy;
+  int64_t dy_bs, dy_ts;
+  const void* dstate_out;
+  void* dx;
+  float* dweight;
+  float* dbias;
+  void* dstate;
+  void* workspace;
+  size_t workspace_bytes;
+} boa_conv_args;
+BOA_API int boa_causal_conv(const boa_conv_args* a, void* stream);
+/* Bytes of workspace for boa_causal_conv_backward (0 on a bad argument). */
+BOA_API size_t boa_causal_conv_workspace_bytes(const boa_conv_args* a);
+BOA_API int boa_causal_conv_backward(const boa_conv_args* a, void* stream);
+/* One token per stream: x is [batch, channels] (x_bs used, length ignored),
+ * `state_out` is both the old window and the new one (updated in place). */
+BOA_API int boa_causal_conv_step(const boa_conv_args* a, void* stream);
+
+/* Selective state space scan with 16 states per channel:
+ *   d = softplus(dt + dt_bias) (or dt + dt_bias),  h_t = exp(d_t A) h_{t-1} + d_t x_t B_t,
+ *   v_t = C_t . h_t + D x_t,  y = v silu(z)  (v without z).
+ * A is [channels, 16]; D, dt_bias [channels] and z may be NULL.  `state`
+ * [batch, channels, 16] fp32 (NULL: zeros) is h before position 0, state_out
+ * (may be NULL) receives h behind every row's last valid position.  lens as in
+ * boa_conv_args.  `checkpoints` (NULL unless a backward call follows;
+ * boa_ssm_checkpoint_bytes) receives the states the backward call restarts
+ * from.  The fields behind `checkpoints` are the backward call's; dz, dD,
+ * ddt_bias, dstate may be NULL where their input is. */
+typedef struct boa_ssm_args {
+  int32_t dtype, batch, length, channels, states, softplus, device, reserved;
+  const void* x;
+  const void* dt;
+  const void* z;
+  const void* B;
+  const void* C;
+  int64_t x_bs, x_ts, dt_bs, dt_ts, z_bs, z_ts, B_bs, B_ts, C_bs, C_ts;
+  const float* A;
+  const float* D;
+  const float* dt_bias;
+  const float* state;
+  const int32_t* lens;
+  void* y;
+  float* state_out;
+  float* checkpoints;
+  const void* dy;
+  int64_t dy_bs, dy_ts;
+  const float* dstate_out;
+  void* dx;
+  void* ddt;
+  void* dz;
+  void* dB;
+  void* dC;
+  float* dA;
+  float* dD;
+  float* ddt_bias;
+  float* dstate;
+  void* workspace;
+  size_t workspace_bytes;
+} boa_ssm_args;
+BOA_API size_t boa_ssm_checkpoint_bytes(const boa_ssm_args* a);
+/* Bytes of workspace for boa_ssm_scan (backward = 0) or boa_ssm_scan_backward. */
+BOA_API size_t boa_ssm_workspace_bytes(const boa_ssm_args* a, int backward);
+BOA_API int boa_ssm_scan(const boa_ssm_args* a, void* stream);
+BOA_API int boa_ssm_scan_backward(const boa_ssm_args* a, void* stream);
+/* One token per stream: x, dt, z, B, C are [batch, ...] rows (*_bs used,
+ * length ignored); `state_out` is updated in place. */
+BOA_API int boa_ssm_step(const boa_ssm_args* a, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Diagnostics (no reference counterpart).                                  */
 /* ------------------------------------------------------------------------ */
 /* Failure-path check (no reference counterpart): launches one thread that
