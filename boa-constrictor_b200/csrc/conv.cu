@@ -25,8 +25,6 @@ struct ConvRuns {
   int64_t run_blocks;
 };
 
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
-
 // Row t of the sequence with its past: x at t >= 0, the state (or zeros) before.
 template <typename T, int V, int K>
 __device__ __forceinline__ void past_row(const T* x, int64_t ts, const T* state, int channels, int t, float (&v)[V]) {

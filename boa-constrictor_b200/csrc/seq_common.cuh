@@ -42,6 +42,63 @@ __device__ __forceinline__ void store_f(T* p, const float (&in)[V]) {
   *reinterpret_cast<Vec<T, V>*>(p) = r;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp(1.0f + ex2(-kLog2e * v)); }
+
+// softplus(v) = max(v, 0) + log(1 + u), u = exp(-|v|), with
+// log(1 + u) = 2 artanh(s), s = u / (2 + u) <= 1/3, and artanh(s) / s a minimax
+// polynomial in s^2 (relative error 4e-9): exact to a few units in the last
+// place for every v, where log2 of a rounded 1 + u would lose small u.
+__device__ __forceinline__ float softplus_f(float v, float& u) {
+  u = ex2(-kLog2e * fabsf(v));
+  const float s = u * rcp(2.0f + u), w = s * s;
+  float p = fmaf(0.14089173f, w, 0.13980299f);
+  p = fmaf(p, w, 0.20012455f);
+  p = fmaf(p, w, 0.33333158f);
+  p = fmaf(p, w, 1.0f);
+  return fmaxf(v, 0.0f) + 2.0f * s * p;
+}
+
+// Pairs of fp32 in one 64-bit register: one instruction for two operations.
+struct f2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ f2 pack(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(f2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ f2 ex2_2(f2 a) {
+  const float2 t = unpack(a);
+  return pack(ex2(t.x), ex2(t.y));
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

@@ -17,6 +17,8 @@
 // taken.  The backward call does the same with the gradient of the state, in
 // reverse, and restarts h from checkpoints every 8 tokens that the forward call
 // leaves.
+#include <cstring>
+
 #include "seq_common.cuh"
 
 namespace boa {
@@ -30,48 +32,77 @@ constexpr int kTile = 16;         // tokens a forward tile
 constexpr int kBack = 8;          // tokens a backward tile, and between checkpoints
 constexpr int kPitch = 40;        // floats of a staged row: 8 mod 32, so 4 rows x 8 channels hit 32 banks
 constexpr int kPasses = 8;        // channel passes of a backward block
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float softplus_of(float v) { return v > 20.0f ? v : log1pf(expf(v)); }
-__device__ __forceinline__ float sigmoid_of(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 
 __device__ __forceinline__ int row_len(const boa_ssm_args& a, int b) {
   return a.lens ? min(max(a.lens[b], 0), a.length) : a.length;
 }
 
-// Two neighbouring channels of a token row; zeros where the token or the
-// channel does not exist.  `pair`: every row starts on a pair boundary.
-template <typename T>
-__device__ __forceinline__ Vec<T, 2> load_pair(const T* row, int c, int E, bool live, bool pair) {
-  Vec<T, 2> r;
-  r.v[0] = from_f<T>(0.0f);
-  r.v[1] = from_f<T>(0.0f);
-  if (live) {
-    if (pair) {
-      if (c < E) r = *reinterpret_cast<const Vec<T, 2>*>(row + c);
+// V neighbouring elements of a token row as loaded, zeros where the token or the
+// channel does not exist.  VEC (every row starts on whole vectors): one access,
+// kept as the words it arrives in, so that nothing waits for a load before the
+// values are used a tile later.
+template <typename T, int V, bool VEC>
+struct Row {
+  static constexpr int kWords = VEC ? V * (int)sizeof(T) / 4 : V;
+  uint32_t w[kWords];
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[j]);
     } else {
-      if (c < E) r.v[0] = row[c];
-      if (c + 1 < E) r.v[1] = row[c + 1];
+      const unsigned short h = VEC ? (unsigned short)(w[j / 2] >> (16 * (j & 1))) : (unsigned short)w[j];
+      T t;
+      memcpy(&t, &h, 2);
+      return to_f(t);
     }
   }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store_pair(T* row, int c, int E, float v0, float v1, bool pair) {
-  if (pair) {
-    if (c < E) {
-      const float v[2] = {v0, v1};
-      store_f<T, 2>(row + c, v);
+  __device__ __forceinline__ void load(const T* p, int c, int E, bool live) {
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) w[j] = 0;
+    if constexpr (VEC) {
+      if (live && c < E) {
+        if constexpr (kWords == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+        if constexpr (kWords == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          w[0] = v.x;
+          w[1] = v.y;
+        }
+        if constexpr (kWords == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p);
+          w[0] = v.x;
+          w[1] = v.y;
+          w[2] = v.z;
+          w[3] = v.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (live && c + j < E) {
+          if constexpr (sizeof(T) == 4) w[j] = reinterpret_cast<const uint32_t*>(p)[j];
+          else w[j] = reinterpret_cast<const unsigned short*>(p)[j];
+        }
     }
+  }
+};
+template <typename T, int V, bool VEC>
+__device__ __forceinline__ void store_row(T* p, int c, int E, const float (&v)[V]) {
+  if constexpr (VEC) {
+    if (c < E) store_f<T, V>(p, v);
   } else {
-    if (c < E) row[c] = from_f<T>(v0);
-    if (c + 1 < E) row[c + 1] = from_f<T>(v1);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (c + j < E) p[j] = from_f<T>(v[j]);
   }
+}
+// Parameters of V channels, zeros beyond the last or without the array.
+template <int V>
+__device__ __forceinline__ void load_params(const float* p, int c, int E, float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = p && c + j < E ? p[c + j] : 0.0f;
+}
+__device__ __forceinline__ float step_of(float raw, bool softplus) {
+  float u;
+  return softplus ? softplus_f(raw, u) : raw;
 }
 
 // Sums of four values over the four lanes of a channel: lane q gets that of v[q].
@@ -86,18 +117,11 @@ __device__ __forceinline__ float quad_sum(const float (&v)[4], int q) {
 struct SsmPlan {
   int cblocks;      // blocks (of 32 channels) of a row
   int parts, part;  // parts of a sequence, tokens of a part
-  bool pair;        // two-element accesses
-};
-
-template <typename T>
-struct RawTile {
-  Vec<T, 2> x[2], dt[2], z[2];
-  float bc[4];
 };
 
 // ------------------------------------------------------------------ forward
 // ENDS: only the part's end state (from zero) and sum of d, into ends / dsum.
-template <typename T, bool ENDS>
+template <typename T, bool ENDS, bool VEC>
 __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const SsmPlan p, float* __restrict__ ends,
                                                      float* __restrict__ dsum) {
   __shared__ __align__(16) float sd[kTile][kPitch], su[kTile][kPitch], sy[kTile][kPitch];
@@ -107,124 +131,129 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
   const int part = (blockIdx.x / p.cblocks) % nparts, b = blockIdx.x / p.cblocks / nparts;
   const int e = e0 + ch;
-  const bool on = e < E;
+  const bool on = e < E, gated = !ENDS && a.z;
   const int len = row_len(a, b);
   const int begin = part * p.part, stop = min(begin + p.part, a.length), end = min(stop, len);
   const int64_t slot = ((int64_t)b * p.parts + part) * E + e;
-  // staging: a thread moves two channels of tokens row and row + 8, and four values of B or C
-  const int row = tid >> 4, c = e0 + 2 * (tid & 15), cl = 2 * (tid & 15);
-  const int brow = tid >> 3, bsub = tid & 7;
-  const T* px = (const T*)a.x + b * a.x_bs;
-  const T* pd = (const T*)a.dt + b * a.dt_bs;
-  const T* pz = a.z ? (const T*)a.z + b * a.z_bs : nullptr;
-  const T* pbc = bsub < 4 ? (const T*)a.B + b * a.B_bs + 4 * bsub : (const T*)a.C + b * a.C_bs + 4 * (bsub - 4);
-  const int64_t bcts = bsub < 4 ? a.B_ts : a.C_ts;
-  const bool want_bc = !ENDS || bsub < 4;
-  float bias[2], Dv[2];
+  // staging: a thread moves four channels of token `row`, and four values of its B or C
+  const int row = tid >> 3, sub = tid & 7, c = e0 + 4 * sub;
+  const bool is_c = sub >= 4;
+  int t = begin + row;
+  const T* px = (const T*)a.x + b * a.x_bs + t * a.x_ts + c;
+  const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
+  const T* pz = (const T*)a.z + b * a.z_bs + t * a.z_ts + c;
+  const T* pbc = is_c ? (const T*)a.C + b * a.C_bs + t * a.C_ts + 4 * (sub - 4)
+                      : (const T*)a.B + b * a.B_bs + t * a.B_ts + 4 * sub;
+  const int64_t bcts = is_c ? a.C_ts : a.B_ts;
+  T* py = (T*)a.y + ((int64_t)b * a.length + t) * E + c;
+  float bias[4], Dv[4];
+  load_params<4>(a.dt_bias, c, E, bias);
+  load_params<4>(a.D, c, E, Dv);
+  f2 A2[2], h[2];
+  {
+    float v[kQ], s[kQ];
+    const float* s0 = ENDS ? nullptr : p.parts > 1 ? ends + slot * kN : a.state ? a.state + ((int64_t)b * E + e) * kN : nullptr;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    bias[j] = a.dt_bias && c + j < E ? a.dt_bias[c + j] : 0.0f;
-    Dv[j] = a.D && c + j < E ? a.D[c + j] : 0.0f;
-  }
-  float A2[kQ], h[kQ];
-#pragma unroll
-  for (int j = 0; j < kQ; ++j) {
-    A2[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
-    h[j] = 0.0f;
-    if (!ENDS && on) {
-      if (p.parts > 1) h[j] = ends[slot * kN + kQ * q + j];
-      else if (a.state) h[j] = a.state[((int64_t)b * E + e) * kN + kQ * q + j];
+    for (int j = 0; j < kQ; ++j) {
+      v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+      s[j] = on && s0 ? s0[kQ * q + j] : 0.0f;
     }
+    A2[0] = pack(v[0], v[1]);
+    A2[1] = pack(v[2], v[3]);
+    h[0] = pack(s[0], s[1]);
+    h[1] = pack(s[2], s[3]);
   }
+  const int nck = (a.length + kBack - 1) / kBack;
+  float* ck = !ENDS && a.checkpoints && on
+                  ? a.checkpoints + (((int64_t)b * nck + begin / kBack) * E + e) * kN + kQ * q : nullptr;
   float total = 0.0f;
-  RawTile<T> r;
-  auto fetch = [&](int t0) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = t0 + row + 8 * i;
-      const bool live = t < end;
-      r.x[i] = load_pair<T>(px + (int64_t)t * a.x_ts, c, E, live, p.pair);
-      r.dt[i] = load_pair<T>(pd + (int64_t)t * a.dt_ts, c, E, live, p.pair);
-      if (!ENDS && pz) r.z[i] = load_pair<T>(pz + (int64_t)t * a.z_ts, c, E, live, p.pair);
-    }
-    const int t = t0 + brow;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r.bc[j] = want_bc && t < end ? to_f(pbc[(int64_t)t * bcts + j]) : 0.0f;
+  Row<T, 4, VEC> rx, rd, rz, rb;
+  auto fetch = [&]() {
+    const bool live = t < end;
+    rx.load(px, c, E, live);
+    rd.load(pd, c, E, live);
+    if (gated) rz.load(pz, c, E, live);
+    rb.load(pbc, 0, 4, live && !(ENDS && is_c));
+    px += kTile * a.x_ts;
+    pd += kTile * a.dt_ts;
+    pz += kTile * a.z_ts;
+    pbc += kTile * bcts;
   };
-  if (begin < end) fetch(begin);
+  if (begin < end) fetch();
   for (int t0 = begin; t0 < end; t0 += kTile) {
-    float xs[2][2], zs[2][2];
+    float xs[4], zs[4], d[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const bool live = t0 + row + 8 * i < end && c + j < E;
-        const float raw = to_f(r.dt[i].v[j]) + bias[j];
-        const float d = live ? (a.softplus ? softplus_of(raw) : raw) : 0.0f;
-        xs[i][j] = to_f(r.x[i].v[j]);
-        zs[i][j] = !ENDS && pz ? to_f(r.z[i].v[j]) : 0.0f;
-        sd[row + 8 * i][cl + j] = d;
-        su[row + 8 * i][cl + j] = d * xs[i][j];
-      }
-    *reinterpret_cast<float4*>(&sbc[brow][4 * bsub]) = make_float4(r.bc[0], r.bc[1], r.bc[2], r.bc[3]);
+    for (int j = 0; j < 4; ++j) {
+      xs[j] = rx.get(j);
+      zs[j] = gated ? rz.get(j) : 0.0f;
+      d[j] = t < end ? step_of(rd.get(j) + bias[j], a.softplus) : 0.0f;
+    }
+    *reinterpret_cast<float4*>(&sd[row][4 * sub]) = make_float4(d[0], d[1], d[2], d[3]);
+    *reinterpret_cast<float4*>(&su[row][4 * sub]) = make_float4(d[0] * xs[0], d[1] * xs[1], d[2] * xs[2], d[3] * xs[3]);
+    *reinterpret_cast<float4*>(&sbc[row][4 * sub]) = make_float4(rb.get(0), rb.get(1), rb.get(2), rb.get(3));
+    const bool mine = t < stop, live = t < end;
+    t += kTile;
     __syncthreads();
-    if (t0 + kTile < end) fetch(t0 + kTile);
+    if (t0 + kTile < end) fetch();
 #pragma unroll
     for (int u = 0; u < kTile; u += 4) {
       float yp[4];
-      if (!ENDS && a.checkpoints && u % kBack == 0 && on && t0 + u < end) {
-        const int64_t nck = (a.length + kBack - 1) / kBack;
-        *reinterpret_cast<float4*>(a.checkpoints + (((int64_t)b * nck + (t0 + u) / kBack) * E + e) * kN + kQ * q) =
-            make_float4(h[0], h[1], h[2], h[3]);
+      if (!ENDS && u % kBack == 0 && ck && t0 + u < end) {
+        *reinterpret_cast<ulonglong2*>(ck) = make_ulonglong2(h[0].v, h[1].v);
+        ck += (int64_t)E * kN;
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float d = sd[u + k][ch], du = su[u + k][ch];
-        const float4 B4 = *reinterpret_cast<const float4*>(&sbc[u + k][kQ * q]);
-        const float Bv[4] = {B4.x, B4.y, B4.z, B4.w};
-#pragma unroll
-        for (int j = 0; j < kQ; ++j) h[j] = fmaf(ex2(d * A2[j]), h[j], du * Bv[j]);
+        const float dk = sd[u + k][ch], uk = su[u + k][ch];
+        const f2 dd = pack(dk, dk), uu = pack(uk, uk);
+        const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sbc[u + k][kQ * q]);
+        h[0] = fma2(ex2_2(mul2(dd, A2[0])), h[0], mul2(uu, f2{B.x}));
+        h[1] = fma2(ex2_2(mul2(dd, A2[1])), h[1], mul2(uu, f2{B.y}));
         if constexpr (ENDS) {
-          total += d;
+          total += dk;
         } else {
-          const float4 C4 = *reinterpret_cast<const float4*>(&sbc[u + k][kN + kQ * q]);
-          yp[k] = fmaf(C4.x, h[0], fmaf(C4.y, h[1], fmaf(C4.z, h[2], C4.w * h[3])));
+          const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sbc[u + k][kN + kQ * q]);
+          const float2 y = unpack(fma2(f2{C.x}, h[0], mul2(f2{C.y}, h[1])));
+          yp[k] = y.x + y.y;
         }
       }
       if constexpr (!ENDS) sy[u + q][ch] = quad_sum(yp, q);
     }
     __syncthreads();
     if constexpr (!ENDS) {
+      if (mine) {
+        float o[4];
+        const float4 v = *reinterpret_cast<const float4*>(&sy[row][4 * sub]);
+        const float vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = t0 + row + 8 * i;
-        if (t < stop) {
-          float o[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            o[j] = fmaf(Dv[j], xs[i][j], sy[row + 8 * i][cl + j]);
-            if (pz) o[j] *= zs[i][j] * sigmoid_of(zs[i][j]);
-            if (t >= end) o[j] = 0.0f;
-          }
-          store_pair<T>((T*)a.y + ((int64_t)b * a.length + t) * E, c, E, o[0], o[1], p.pair);
+        for (int j = 0; j < 4; ++j) {
+          o[j] = fmaf(Dv[j], xs[j], vv[j]);
+          if (gated) o[j] *= zs[j] * sigmoid_f(zs[j]);
+          if (!live) o[j] = 0.0f;
         }
+        store_row<T, 4, VEC>(py, c, E, o);
       }
+      py += (int64_t)kTile * E;
     }
   }
   if constexpr (ENDS) {
     if (on) {
-      *reinterpret_cast<float4*>(ends + slot * kN + kQ * q) = make_float4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(h[0].v, h[1].v);
       if (q == 0) dsum[slot] = total;
     }
   } else {
-    // tiles wholly behind the row's end
-    const int done = begin + (max(end - begin, 0) + kTile - 1) / kTile * kTile;
-    for (int t = done + row; t < stop; t += 8)
-      store_pair<T>((T*)a.y + ((int64_t)b * a.length + t) * E, c, E, 0.0f, 0.0f, p.pair);
+    const float zero[4] = {};
+    for (; t < stop; t += kTile) {   // tiles wholly behind the row's end
+      store_row<T, 4, VEC>(py, c, E, zero);
+      py += (int64_t)kTile * E;
+    }
     if (a.state_out && part == p.parts - 1 && on) {
       float* so = a.state_out + ((int64_t)b * E + e) * kN + kQ * q;
-#pragma unroll
-      for (int j = 0; j < kQ; ++j) so[j] = h[j];
+      const float2 lo = unpack(h[0]), hi = unpack(h[1]);
+      so[0] = lo.x;
+      so[1] = lo.y;
+      so[2] = hi.x;
+      so[3] = hi.y;
     }
   }
 }
@@ -232,32 +261,40 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
 // Chains the parts of every (row, channel, state): ends[] becomes the value
 // each part starts from.  Forward: from the first part with h; backward
 // (`reverse`): from the last part with the gradient of the state.
-static __global__ void __launch_bounds__(256) k_ssm_join(int64_t n, int E, int parts, const float* __restrict__ A,
-                                                         const float* __restrict__ first, float* __restrict__ ends,
+static __global__ void __launch_bounds__(128) k_ssm_join(int64_t n, int E, int parts, const float* __restrict__ A,
+                                                         const float* __restrict__ first, float* ends,
                                                          const float* __restrict__ dsum, bool reverse) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x;
   if (i >= n) return;
   const int64_t en = (int64_t)E * kN;
   const int64_t b = i / en, r = i % en;
   const float A2 = A[r] * kLog2e;
   float carry = first ? first[i] : 0.0f;
-  for (int k = 0; k < parts; ++k) {
-    const int s = reverse ? parts - 1 - k : k;
-    const int64_t at = (b * parts + s) * en + r;
-    float own = 0.0f, decay = 0.0f;
-    if (k < parts - 1) {
-      own = ends[at];
-      decay = ex2(A2 * dsum[(b * parts + s) * E + r / kN]);
+  const int64_t step = reverse ? -1 : 1;
+  int64_t s = b * parts + (reverse ? parts - 1 : 0);
+  constexpr int kAhead = 16;   // parts whose loads are in flight together
+  for (int k0 = 0; k0 < parts; k0 += kAhead) {
+    float own[kAhead], sum[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const bool have = k0 + j < parts - 1;
+      own[j] = have ? ends[(s + j * step) * en + r] : 0.0f;
+      sum[j] = have ? dsum[(s + j * step) * E + r / kN] : 0.0f;
     }
-    ends[at] = carry;
-    carry = fmaf(decay, carry, own);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (k0 + j < parts) {
+        ends[(s + j * step) * en + r] = carry;
+        carry = fmaf(ex2(A2 * sum[j]), carry, own[j]);
+      }
+    s += kAhead * step;
   }
 }
 
 // ----------------------------------------------------------------- backward
 // The gradient of the state that a part passes on to the part before it, from
 // a zero start at its end, and the part's sum of d.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_args a, const SsmPlan p,
                                                                float* __restrict__ ends, float* __restrict__ dsum) {
   __shared__ __align__(16) float sd[kTile][kPitch], sg[kTile][kPitch];
@@ -266,70 +303,71 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
   const int part = 1 + (blockIdx.x / p.cblocks) % (p.parts - 1), b = blockIdx.x / p.cblocks / (p.parts - 1);
   const int e = e0 + ch;
-  const bool on = e < E;
+  const bool on = e < E, gated = a.z;
   const int begin = part * p.part, end = min(min(begin + p.part, a.length), row_len(a, b));
   const int64_t slot = ((int64_t)b * p.parts + part) * E + e;
-  const int row = tid >> 4, c = e0 + 2 * (tid & 15), cl = 2 * (tid & 15);
-  const int brow = tid >> 3, bsub = tid & 7;
-  const T* pg = (const T*)a.dy + b * a.dy_bs;
-  const T* pd = (const T*)a.dt + b * a.dt_bs;
-  const T* pz = a.z ? (const T*)a.z + b * a.z_bs : nullptr;
-  const T* pc = (const T*)a.C + b * a.C_bs + 4 * (bsub & 3);
-  float bias[2], A2[kQ], g4[kQ] = {};
-#pragma unroll
-  for (int j = 0; j < 2; ++j) bias[j] = a.dt_bias && c + j < E ? a.dt_bias[c + j] : 0.0f;
-#pragma unroll
-  for (int j = 0; j < kQ; ++j) A2[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
-  float total = 0.0f;
-  RawTile<T> r;   // x holds dy
-  auto fetch = [&](int t0) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = t0 + row + 8 * i;
-      const bool live = t < end;
-      r.x[i] = load_pair<T>(pg + (int64_t)t * a.dy_ts, c, E, live, p.pair);
-      r.dt[i] = load_pair<T>(pd + (int64_t)t * a.dt_ts, c, E, live, p.pair);
-      if (pz) r.z[i] = load_pair<T>(pz + (int64_t)t * a.z_ts, c, E, live, p.pair);
-    }
-    const int t = t0 + brow;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r.bc[j] = bsub < 4 && t < end ? to_f(pc[(int64_t)t * a.C_ts + j]) : 0.0f;
-  };
+  const int row = tid >> 3, sub = tid & 7, c = e0 + 4 * sub;
   const int tiles = (max(end - begin, 0) + kTile - 1) / kTile;
-  if (tiles) fetch(begin + (tiles - 1) * kTile);
+  int t = begin + (tiles - 1) * kTile + row;
+  const T* pg = (const T*)a.dy + b * a.dy_bs + t * a.dy_ts + c;
+  const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
+  const T* pz = (const T*)a.z + b * a.z_bs + t * a.z_ts + c;
+  const T* pc = (const T*)a.C + b * a.C_bs + t * a.C_ts + 4 * sub;   // lanes with sub < 4
+  float bias[4];
+  load_params<4>(a.dt_bias, c, E, bias);
+  f2 A2[2], g2[2] = {pack(0.f, 0.f), pack(0.f, 0.f)};
+  {
+    float v[kQ];
+#pragma unroll
+    for (int j = 0; j < kQ; ++j) v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+    A2[0] = pack(v[0], v[1]);
+    A2[1] = pack(v[2], v[3]);
+  }
+  float total = 0.0f;
+  Row<T, 4, VEC> rg, rd, rz, rc;
+  auto fetch = [&]() {
+    const bool live = t < end;
+    rg.load(pg, c, E, live);
+    rd.load(pd, c, E, live);
+    if (gated) rz.load(pz, c, E, live);
+    rc.load(pc, 0, 4, live && sub < 4);
+    pg -= kTile * a.dy_ts;
+    pd -= kTile * a.dt_ts;
+    pz -= kTile * a.z_ts;
+    pc -= kTile * a.C_ts;
+  };
+  if (tiles) fetch();
   for (int k = tiles - 1; k >= 0; --k) {
-    const int t0 = begin + k * kTile;
+    float d[4], g[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const bool live = t0 + row + 8 * i < end && c + j < E;
-        const float raw = to_f(r.dt[i].v[j]) + bias[j];
-        float g = to_f(r.x[i].v[j]);
-        if (pz) {
-          const float z = to_f(r.z[i].v[j]);
-          g *= z * sigmoid_of(z);
-        }
-        sd[row + 8 * i][cl + j] = live ? (a.softplus ? softplus_of(raw) : raw) : 0.0f;
-        sg[row + 8 * i][cl + j] = live ? g : 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      g[j] = rg.get(j);
+      if (gated) {
+        const float z = rz.get(j);
+        g[j] *= z * sigmoid_f(z);
       }
-    if (bsub < 4)
-      *reinterpret_cast<float4*>(&sc[brow][4 * bsub]) = make_float4(r.bc[0], r.bc[1], r.bc[2], r.bc[3]);
+      d[j] = t < end ? step_of(rd.get(j) + bias[j], a.softplus) : 0.0f;
+    }
+    *reinterpret_cast<float4*>(&sd[row][4 * sub]) = make_float4(d[0], d[1], d[2], d[3]);
+    *reinterpret_cast<float4*>(&sg[row][4 * sub]) = make_float4(g[0], g[1], g[2], g[3]);
+    if (sub < 4)
+      *reinterpret_cast<float4*>(&sc[row][4 * sub]) = make_float4(rc.get(0), rc.get(1), rc.get(2), rc.get(3));
+    t -= kTile;
     __syncthreads();
-    if (k > 0) fetch(t0 - kTile);
+    if (k > 0) fetch();
 #pragma unroll
-    for (int t = kTile - 1; t >= 0; --t) {
-      const float d = sd[t][ch], g = sg[t][ch];
-      const float4 C4 = *reinterpret_cast<const float4*>(&sc[t][kQ * q]);
-      const float Cv[4] = {C4.x, C4.y, C4.z, C4.w};
-#pragma unroll
-      for (int j = 0; j < kQ; ++j) g4[j] = ex2(d * A2[j]) * fmaf(Cv[j], g, g4[j]);
-      total += d;
+    for (int i = kTile - 1; i >= 0; --i) {
+      const float dk = sd[i][ch], gk = sg[i][ch];
+      const f2 dd = pack(dk, dk), gg = pack(gk, gk);
+      const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sc[i][kQ * q]);
+      g2[0] = mul2(ex2_2(mul2(dd, A2[0])), fma2(f2{C.x}, gg, g2[0]));
+      g2[1] = mul2(ex2_2(mul2(dd, A2[1])), fma2(f2{C.y}, gg, g2[1]));
+      total += dk;
     }
     __syncthreads();
   }
   if (on) {
-    *reinterpret_cast<float4*>(ends + slot * kN + kQ * q) = make_float4(g4[0], g4[1], g4[2], g4[3]);
+    *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(g2[0].v, g2[1].v);
     if (q == 0) dsum[slot] = total;
   }
 }
@@ -344,9 +382,9 @@ struct BackSmem {
   __host__ __device__ static constexpr int floats(int passes) { return carry + passes * kCh * per_channel; }
 };
 
-template <typename T>
+template <typename T, bool VEC>
 struct RawBack {
-  Vec<T, 2> x, dt, z, g;
+  Row<T, 2, VEC> x, dt, z, g;
   float4 h;
 };
 
@@ -355,7 +393,7 @@ struct RawBack {
 // checkpoint (a and h stay in registers), then runs the gradient backwards.
 // dB and dC of the tile gather over the passes in registers and are summed
 // over the block's lanes and warps once a tile.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSsmThreads, 3)
     k_ssm_backward(const boa_ssm_args a, const SsmPlan p, int passes, int groups, const float* __restrict__ starts,
                    float* __restrict__ bc_parts, float* __restrict__ param_parts) {
@@ -402,14 +440,14 @@ __global__ void __launch_bounds__(kSsmThreads, 3)
     }
   }
   const int tiles = (max(end - begin, 0) + kBack - 1) / kBack;
-  RawBack<T> r;
+  RawBack<T, VEC> r;
   auto fetch = [&](int t0, int g) {
     const int t = t0 + row, c = e0 + g * kCh + cl;
     const bool live = t < end;
-    r.x = load_pair<T>(px + (int64_t)t * a.x_ts, c, E, live, p.pair);
-    r.dt = load_pair<T>(pd + (int64_t)t * a.dt_ts, c, E, live, p.pair);
-    r.g = load_pair<T>(pg + (int64_t)t * a.dy_ts, c, E, live, p.pair);
-    if (pz) r.z = load_pair<T>(pz + (int64_t)t * a.z_ts, c, E, live, p.pair);
+    r.x.load(px + (int64_t)t * a.x_ts + c, c, E, live);
+    r.dt.load(pd + (int64_t)t * a.dt_ts + c, c, E, live);
+    r.g.load(pg + (int64_t)t * a.dy_ts + c, c, E, live);
+    if (pz) r.z.load(pz + (int64_t)t * a.z_ts + c, c, E, live);
     const int e = e0 + g * kCh + ch;
     r.h = make_float4(0.f, 0.f, 0.f, 0.f);
     if (e < E)
@@ -436,15 +474,16 @@ __global__ void __launch_bounds__(kSsmThreads, 3)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const bool live = in_row && c + j < E;
-        const float raw = to_f(r.dt.v[j]) + (a.dt_bias && c + j < E ? a.dt_bias[c + j] : 0.0f);
+        float u = 0.0f;
+        const float raw = r.dt.get(j) + (a.dt_bias && c + j < E ? a.dt_bias[c + j] : 0.0f);
         Dv[j] = a.D && c + j < E ? a.D[c + j] : 0.0f;
-        dv[j] = live ? (a.softplus ? softplus_of(raw) : raw) : 0.0f;
-        sig[j] = a.softplus ? sigmoid_of(raw) : 1.0f;
-        xv[j] = to_f(r.x.v[j]);
-        gv[j] = to_f(r.g.v[j]);
+        dv[j] = live ? (a.softplus ? softplus_f(raw, u) : raw) : 0.0f;
+        sig[j] = a.softplus ? (raw >= 0.0f ? 1.0f : u) * rcp(1.0f + u) : 1.0f;
+        xv[j] = r.x.get(j);
+        gv[j] = r.g.get(j);
         dzf[j] = 0.0f;
         if (pz) {
-          const float z = to_f(r.z.v[j]), s = sigmoid_of(z);
+          const float z = r.z.get(j), s = sigmoid_f(z);
           dzf[j] = gv[j] * (s * (1.0f + z * (1.0f - s)));
           gv[j] *= z * s;
         }
@@ -530,9 +569,9 @@ __global__ void __launch_bounds__(kSsmThreads, 3)
           *accb += od[j];
         }
         const int64_t o = (orow + t0 + row) * E;
-        store_pair<T>((T*)a.dx + o, c, E, ox[0], ox[1], p.pair);
-        store_pair<T>((T*)a.ddt + o, c, E, od[0], od[1], p.pair);
-        if (pz) store_pair<T>((T*)a.dz + o, c, E, oz[0], oz[1], p.pair);
+        store_row<T, 2, VEC>((T*)a.dx + o + c, c, E, ox);
+        store_row<T, 2, VEC>((T*)a.ddt + o + c, c, E, od);
+        if (pz) store_row<T, 2, VEC>((T*)a.dz + o + c, c, E, oz);
       }
     }
     // the tile's dB and dC over the warp's 8 channels: lane bits 4, 3, 2 pick C, and the state within the lane's four
@@ -560,13 +599,14 @@ __global__ void __launch_bounds__(kSsmThreads, 3)
     }
   }
   // tiles wholly behind the row's end
+  const float zero2[2] = {};
   for (int t = begin + tiles * kBack + row; t < stop; t += kBack) {
     const int64_t o = (orow + t) * E;
     for (int g = 0; g < np; ++g) {
       const int c = e0 + g * kCh + cl;
-      store_pair<T>((T*)a.dx + o, c, E, 0.0f, 0.0f, p.pair);
-      store_pair<T>((T*)a.ddt + o, c, E, 0.0f, 0.0f, p.pair);
-      if (pz) store_pair<T>((T*)a.dz + o, c, E, 0.0f, 0.0f, p.pair);
+      store_row<T, 2, VEC>((T*)a.dx + o + c, c, E, zero2);
+      store_row<T, 2, VEC>((T*)a.ddt + o + c, c, E, zero2);
+      if (pz) store_row<T, 2, VEC>((T*)a.dz + o + c, c, E, zero2);
     }
     float* bc = bc_parts + (((int64_t)group * a.batch + b) * a.length + t) * 2 * kN + 2 * (tid & 15);
     bc[0] = 0.0f;
@@ -632,7 +672,7 @@ __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
   const T* C = (const T*)a.C + b * a.C_bs + kQ * q;
   const float x = to_f(((const T*)a.x)[b * a.x_bs + e]);
   const float raw = to_f(((const T*)a.dt)[b * a.dt_bs + e]) + (a.dt_bias ? a.dt_bias[e] : 0.0f);
-  const float d = a.softplus ? softplus_of(raw) : raw, du = d * x;
+  const float d = step_of(raw, a.softplus), du = d * x;
   float h[4] = {h4.x, h4.y, h4.z, h4.w};
   const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
   float v = 0.0f;
@@ -648,7 +688,7 @@ __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
     if (a.D) v = fmaf(a.D[e], x, v);
     if (a.z) {
       const float z = to_f(((const T*)a.z)[b * a.z_bs + e]);
-      v *= z * sigmoid_of(z);
+      v *= z * sigmoid_f(z);
     }
     ((T*)a.y)[be] = from_f<T>(v);
   }
@@ -687,42 +727,47 @@ static int back_groups(const boa_ssm_args& a) {
 static SsmPlan plan_forward(const boa_ssm_args& a) { return ssm_plan(a, (a.channels + kCh - 1) / kCh, 888, 1776); }
 static SsmPlan plan_backward(const boa_ssm_args& a) { return ssm_plan(a, back_groups(a), 444, 1776); }
 
-static bool even(int64_t v) { return v % 2 == 0; }
-
-static bool ssm_pair(const boa_ssm_args& a, bool backward) {
-  const size_t s = a.dtype == BOA_DTYPE_F32 ? 8 : 4;
-  bool ok = even(a.channels) && even(a.x_bs) && even(a.x_ts) && even(a.dt_bs) && even(a.dt_ts) && aligned(a.x, s) &&
-            aligned(a.dt, s);
-  if (a.z) ok = ok && even(a.z_bs) && even(a.z_ts) && aligned(a.z, s);
-  if (!backward) return ok && aligned(a.y, s);
-  return ok && even(a.dy_bs) && even(a.dy_ts) && aligned(a.dy, s) && aligned(a.dx, s) && aligned(a.ddt, s) &&
-         aligned(a.dz, s);
+// Vector accesses where every row of every tensor starts on four elements.
+static bool row_vec(const void* p, int64_t bs, int64_t ts, size_t size) {
+  return bs % 4 == 0 && ts % 4 == 0 && aligned(p, 4 * size);
+}
+static bool ssm_vec(const boa_ssm_args& a, bool backward) {
+  const size_t s = a.dtype == BOA_DTYPE_F32 ? 4 : 2;
+  const bool ok = a.channels % 4 == 0 && row_vec(a.x, a.x_bs, a.x_ts, s) && row_vec(a.dt, a.dt_bs, a.dt_ts, s) &&
+                  row_vec(a.B, a.B_bs, a.B_ts, s) && row_vec(a.C, a.C_bs, a.C_ts, s) &&
+                  (!a.z || row_vec(a.z, a.z_bs, a.z_ts, s));
+  if (!backward) return ok && aligned(a.y, 4 * s);
+  return ok && row_vec(a.dy, a.dy_bs, a.dy_ts, s) && aligned(a.dx, 4 * s) && aligned(a.ddt, 4 * s) &&
+         aligned(a.dz, 4 * s);
 }
 
 static size_t ends_floats(const boa_ssm_args& a, const SsmPlan& p) {
   return p.parts > 1 ? (size_t)a.batch * p.parts * a.channels * (kN + 1) : 0;
 }
 
-template <typename T>
-static int ssm_forward(const boa_ssm_args& a, cudaStream_t s) {
-  SsmPlan p = plan_forward(a);
-  p.pair = ssm_pair(a, false);
+template <typename T, bool VEC>
+static int ssm_forward_t(const boa_ssm_args& a, cudaStream_t s) {
+  const SsmPlan p = plan_forward(a);
   float* ends = (float*)a.workspace;
   float* dsum = ends + (size_t)a.batch * p.parts * a.channels * kN;
   if (p.parts > 1) {
-    k_ssm<T, true><<<(unsigned)((int64_t)p.cblocks * (p.parts - 1) * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
+    k_ssm<T, true, VEC><<<(unsigned)((int64_t)p.cblocks * (p.parts - 1) * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
     const int64_t n = (int64_t)a.batch * a.channels * kN;
-    k_ssm_join<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(n, a.channels, p.parts, a.A, a.state, ends, dsum, false);
+    k_ssm_join<<<(unsigned)((n + 127) / 128), 128, 0, s>>>(n, a.channels, p.parts, a.A, a.state, ends, dsum, false);
   }
-  k_ssm<T, false><<<(unsigned)((int64_t)p.cblocks * p.parts * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
+  k_ssm<T, false, VEC><<<(unsigned)((int64_t)p.cblocks * p.parts * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
 }
 
 template <typename T>
-static int ssm_backward(const boa_ssm_args& a, cudaStream_t s) {
-  SsmPlan p = plan_backward(a);
-  p.pair = ssm_pair(a, true);
+static int ssm_forward(const boa_ssm_args& a, cudaStream_t s) {
+  return ssm_vec(a, false) ? ssm_forward_t<T, true>(a, s) : ssm_forward_t<T, false>(a, s);
+}
+
+template <typename T, bool VEC>
+static int ssm_backward_t(const boa_ssm_args& a, cudaStream_t s) {
+  const SsmPlan p = plan_backward(a);
   const int passes = back_passes(a), groups = back_groups(a);
   float* bc = (float*)a.workspace;
   float* params = bc + (size_t)groups * a.batch * a.length * 2 * kN;
@@ -731,14 +776,14 @@ static int ssm_backward(const boa_ssm_args& a, cudaStream_t s) {
   ends = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ends) + 15) & ~uintptr_t(15));
   float* dsum = ends + (size_t)a.batch * p.parts * a.channels * kN;
   if (p.parts > 1) {
-    k_ssm_back_ends<T>
+    k_ssm_back_ends<T, VEC>
         <<<(unsigned)((int64_t)p.cblocks * (p.parts - 1) * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
     const int64_t n = (int64_t)a.batch * a.channels * kN;
-    k_ssm_join<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(n, a.channels, p.parts, a.A, a.dstate_out, ends, dsum, true);
+    k_ssm_join<<<(unsigned)((n + 127) / 128), 128, 0, s>>>(n, a.channels, p.parts, a.A, a.dstate_out, ends, dsum, true);
   }
   const int smem = BackSmem::floats(passes) * (int)sizeof(float);
-  BOA_CUDA(cudaFuncSetAttribute(k_ssm_backward<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  k_ssm_backward<T><<<(unsigned)((int64_t)groups * p.parts * a.batch), kSsmThreads, smem, s>>>(a, p, passes, groups,
+  BOA_CUDA(cudaFuncSetAttribute(k_ssm_backward<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  k_ssm_backward<T, VEC><<<(unsigned)((int64_t)groups * p.parts * a.batch), kSsmThreads, smem, s>>>(a, p, passes, groups,
                                                                                              ends, bc, params);
   const int64_t rows = (int64_t)a.batch * a.length, n = rows * 2 * kN;
   if (n > 0)
@@ -748,6 +793,11 @@ static int ssm_backward(const boa_ssm_args& a, cudaStream_t s) {
                                               a.channels * (kN + 1), a.dA, a.dD, a.ddt_bias);
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
+}
+
+template <typename T>
+static int ssm_backward(const boa_ssm_args& a, cudaStream_t s) {
+  return ssm_vec(a, true) ? ssm_backward_t<T, true>(a, s) : ssm_backward_t<T, false>(a, s);
 }
 
 static int ssm_check(const boa_ssm_args* a, const char* who) {
