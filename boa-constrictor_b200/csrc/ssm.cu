@@ -31,7 +31,7 @@ constexpr int kSsmThreads = 128;
 constexpr int kTile = 16;         // tokens a forward tile
 constexpr int kBack = 8;          // tokens a backward tile, and between checkpoints
 constexpr int kPitch = 40;        // floats of a staged row: 8 mod 32, so 4 rows x 8 channels hit 32 banks
-constexpr int kPasses = 8;        // channel passes of a backward block
+constexpr int kPasses = 8;        // channel passes of a backward block (of 64 channels)
 
 __device__ __forceinline__ int row_len(const boa_ssm_args& a, int b) {
   return a.lens ? min(max(a.lens[b], 0), a.length) : a.length;
@@ -105,13 +105,20 @@ __device__ __forceinline__ float step_of(float raw, bool softplus) {
   return softplus ? softplus_f(raw, u) : raw;
 }
 
+// A warp's 8 channels x 4 state groups: the state group is in lane bits 1 and 2,
+// the channel in bits 0, 3 and 4.  A 16-byte shared load takes 2 wavefronts
+// instead of 4 where lanes that differ in bit 0 alone, or in bit 1 alone, share
+// an address (measured); so both the loads by state (B, C) and those by channel do.
+__device__ __forceinline__ int lane_q(int lane) { return (lane >> 1) & 3; }
+__device__ __forceinline__ int lane_ch(int lane) { return (lane & 1) | ((lane >> 3) << 1); }
+
 // Sums of four values over the four lanes of a channel: lane q gets that of v[q].
 __device__ __forceinline__ float quad_sum(const float (&v)[4], int q) {
   const bool hi = q & 2, odd = q & 1;
   float k0 = hi ? v[2] : v[0], k1 = hi ? v[3] : v[1];
-  k0 += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 2);
-  k1 += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 2);
-  return (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 1);
+  k0 += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 4);
+  k1 += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 4);
+  return (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 2);
 }
 
 struct SsmPlan {
@@ -126,7 +133,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
                                                      float* __restrict__ dsum) {
   __shared__ __align__(16) float sd[kTile][kPitch], su[kTile][kPitch], sy[kTile][kPitch];
   __shared__ __align__(16) float sbc[kTile][2 * kN];
-  const int tid = threadIdx.x, lane = tid & 31, q = lane & 3, ch = (tid >> 5) * 8 + (lane >> 2);
+  const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
   const int nparts = ENDS ? p.parts - 1 : p.parts;
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
   const int part = (blockIdx.x / p.cblocks) % nparts, b = blockIdx.x / p.cblocks / nparts;
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
                                                                float* __restrict__ ends, float* __restrict__ dsum) {
   __shared__ __align__(16) float sd[kTile][kPitch], sg[kTile][kPitch];
   __shared__ __align__(16) float sc[kTile][kN];
-  const int tid = threadIdx.x, lane = tid & 31, q = lane & 3, ch = (tid >> 5) * 8 + (lane >> 2);
+  const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
   const int part = 1 + (blockIdx.x / p.cblocks) % (p.parts - 1), b = blockIdx.x / p.cblocks / (p.parts - 1);
   const int e = e0 + ch;
@@ -372,271 +379,392 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
   }
 }
 
-// Shared memory of the backward kernel, in floats.
+constexpr int kBackCh = 64;                           // channels a backward pass
+constexpr int kBackPitch = 72;                        // 8 mod 32, as kPitch
+constexpr int kBackScan = 256, kBackThreads = kBackScan + 128;
+constexpr int kBackRegs = 168;                        // at launch
+constexpr int kScanRegs = 200, kElementRegs = 104;    // 256 * 200 + 128 * 104 = 384 * 168
+static_assert(kBackScan * kScanRegs + 128 * kElementRegs == kBackThreads * kBackRegs,
+              "the warpgroups share what the block was launched with");
+
+// Shared memory of the backward kernel, in floats.  A slot holds one pass: the
+// staged {d, d, d x, d x} and {g, g} of every token and channel (twice, as the
+// paired operations take them), the channels' states at the tile's start, and
+// the sums the scan warps return.
 struct BackSmem {
-  static constexpr int tile = kBack * kPitch;
-  static constexpr int sd = 0, su = sd + tile, sg = su + tile, s1 = sg + tile, s2 = s1 + tile, sv = s2 + tile,
-                       sbc = sv + tile, red = sbc + kBack * 2 * kN, carry = red + 4 * kBack * 2 * kN;
-  // per channel of the block: dh[16], dA[16], and dD, dbias by staging row
-  static constexpr int per_channel = 2 * kN + 2 * kBack;
-  __host__ __device__ static constexpr int floats(int passes) { return carry + passes * kCh * per_channel; }
+  static constexpr int kSums = kBack * kBackPitch;
+  static constexpr int gg = kBack * kBackCh * 4, h0 = gg + kBack * kBackCh * 2, sums = h0 + kBackCh * kN;
+  static constexpr int kSlot = sums + 3 * kSums;
+  static constexpr int kBc = kBack * 2 * kN;
+  static constexpr int bc = 2 * kSlot, red = bc + 2 * kBc, carry = red + kBackScan / 32 * kBc;
+  // per channel of the block: dh[16], dA[16], A[16] in units of log2, D, dt_bias, and dD, ddt_bias by staging row
+  static constexpr int per_channel = 3 * kN + 2 + 2 * kBack;
+  __host__ __device__ static constexpr int floats(int passes) { return carry + passes * kBackCh * per_channel; }
 };
+static_assert(BackSmem::floats(kPasses) * 4 <= 227 * 1024, "shared memory of a block");
 
-template <typename T, bool VEC>
-struct RawBack {
-  Row<T, 2, VEC> x, dt, z, g;
-  float4 h;
-};
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+enum { kFull = 1, kDone = 3, kScanOnly = 5 };          // barrier ids; kFull and kDone one per slot
 
-// A block takes one part of a row and up to 256 channels, tile by tile from
-// the end, 32 channels a pass.  A pass recomputes h over the tile from its
-// checkpoint (a and h stay in registers), then runs the gradient backwards.
-// dB and dC of the tile gather over the passes in registers and are summed
-// over the block's lanes and warps once a tile.
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ void st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+
+// A block takes one part of a row and up to 512 channels, tile by tile (8
+// tokens) from the end, 64 channels a pass.  The last four warps stage a pass
+// (softplus and the gate, once an element) and finish its gradients; the first
+// eight recompute h over the tile from its checkpoint with a and h in registers
+// and then run the gradient of the state backwards.  The two work on
+// neighbouring passes, two slots of shared memory apart.  dB and dC of a tile
+// gather over its passes in the scan warps' registers (hence setmaxnreg) and
+// are summed over lanes and warps once a tile; with one channel group they are
+// final, else the groups' sums go to bc_parts.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kSsmThreads, 3)
+__global__ void __launch_bounds__(kBackThreads, 1)
     k_ssm_backward(const boa_ssm_args a, const SsmPlan p, int passes, int groups, const float* __restrict__ starts,
                    float* __restrict__ bc_parts, float* __restrict__ param_parts) {
   extern __shared__ __align__(16) float sm[];
   using S = BackSmem;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = lane & 3, ch = warp * 8 + (lane >> 2);
   const int E = a.channels, group = blockIdx.x % groups;
   const int part = (blockIdx.x / groups) % p.parts, b = blockIdx.x / groups / p.parts;
-  const int e0 = group * passes * kCh;
-  const int np = min(passes, (E - e0 + kCh - 1) / kCh);
-  const int len = row_len(a, b);
-  const int begin = part * p.part, stop = min(begin + p.part, a.length), end = min(stop, len);
-  const int nck = (a.length + kBack - 1) / kBack;
-  const int row = tid >> 4, cl = 2 * (tid & 15);
-  const int brow = tid >> 4, bsub = tid & 15;    // two values of B or C
-  const T* px = (const T*)a.x + b * a.x_bs;
-  const T* pd = (const T*)a.dt + b * a.dt_bs;
-  const T* pz = a.z ? (const T*)a.z + b * a.z_bs : nullptr;
-  const T* pg = (const T*)a.dy + b * a.dy_bs;
-  const T* pbc = bsub < 8 ? (const T*)a.B + b * a.B_bs + 2 * bsub : (const T*)a.C + b * a.C_bs + 2 * (bsub - 8);
-  const int64_t bcts = bsub < 8 ? a.B_ts : a.C_ts;
-  const int64_t orow = (int64_t)b * a.length;
-  float* dh_s = sm + S::carry;
-  float* dA_s = dh_s + passes * kCh * kN;
-  float* dD_s = dA_s + passes * kCh * kN;           // [row][channel]
-  float* db_s = dD_s + passes * kCh * kBack;
-  for (int g = 0; g < np; ++g) {
-    const int e = e0 + g * kCh + ch;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (e < E) {
-      if (p.parts > 1) {
-        v = *reinterpret_cast<const float4*>(starts + (((int64_t)b * p.parts + part) * E + e) * kN + kQ * q);
-      } else if (a.dstate_out) {
-        const float* s = a.dstate_out + ((int64_t)b * E + e) * kN + kQ * q;
-        v = make_float4(s[0], s[1], s[2], s[3]);
-      }
-    }
-    *reinterpret_cast<float4*>(dh_s + (g * kCh + ch) * kN + kQ * q) = v;
-    *reinterpret_cast<float4*>(dA_s + (g * kCh + ch) * kN + kQ * q) = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      dD_s[row * passes * kCh + g * kCh + cl + j] = 0.0f;
-      db_s[row * passes * kCh + g * kCh + cl + j] = 0.0f;
-    }
-  }
+  const int width = passes * kBackCh, e0 = group * width;
+  const int np = min(passes, (E - e0 + kBackCh - 1) / kBackCh);
+  const int begin = part * p.part, stop = min(begin + p.part, a.length), end = min(stop, row_len(a, b));
   const int tiles = (max(end - begin, 0) + kBack - 1) / kBack;
-  RawBack<T, VEC> r;
-  auto fetch = [&](int t0, int g) {
-    const int t = t0 + row, c = e0 + g * kCh + cl;
-    const bool live = t < end;
-    r.x.load(px + (int64_t)t * a.x_ts + c, c, E, live);
-    r.dt.load(pd + (int64_t)t * a.dt_ts + c, c, E, live);
-    r.g.load(pg + (int64_t)t * a.dy_ts + c, c, E, live);
-    if (pz) r.z.load(pz + (int64_t)t * a.z_ts + c, c, E, live);
-    const int e = e0 + g * kCh + ch;
-    r.h = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (e < E)
-      r.h = *reinterpret_cast<const float4*>(a.checkpoints + (((int64_t)b * nck + t0 / kBack) * E + e) * kN + kQ * q);
-  };
-  if (tiles) fetch(begin + (tiles - 1) * kBack, 0);
-  for (int k = tiles - 1; k >= 0; --k) {
-    const int t0 = begin + k * kBack;
-    float vB[kBack][kQ], vC[kBack][kQ];
-#pragma unroll
-    for (int t = 0; t < kBack; ++t)
-#pragma unroll
-      for (int j = 0; j < kQ; ++j) vB[t][j] = vC[t][j] = 0.0f;
-    {
-      const int t = t0 + brow;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        sm[S::sbc + brow * 2 * kN + 2 * bsub + j] = t < end ? to_f(pbc[(int64_t)t * bcts + j]) : 0.0f;
-    }
+  float* const dh_s = sm + S::carry;
+  float* const dA_s = dh_s + width * kN;
+  float* const A_s = dA_s + width * kN;
+  float* const D_s = A_s + width * kN;
+  float* const bias_s = D_s + width;
+  float* const dD_s = bias_s + width;                   // [row][channel]
+  float* const db_s = dD_s + width * kBack;
+  const bool gated = a.z;
+  if (threadIdx.x < kBackScan) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kScanRegs));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = lane_q(lane), ch = warp * 8 + lane_ch(lane);
     for (int g = 0; g < np; ++g) {
-      const int c = e0 + g * kCh + cl, e = e0 + g * kCh + ch;
-      const bool in_row = t0 + row < end;
-      float xv[2], dv[2], gv[2], sig[2], dzf[2], Dv[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const bool live = in_row && c + j < E;
-        float u = 0.0f;
-        const float raw = r.dt.get(j) + (a.dt_bias && c + j < E ? a.dt_bias[c + j] : 0.0f);
-        Dv[j] = a.D && c + j < E ? a.D[c + j] : 0.0f;
-        dv[j] = live ? (a.softplus ? softplus_f(raw, u) : raw) : 0.0f;
-        sig[j] = a.softplus ? (raw >= 0.0f ? 1.0f : u) * rcp(1.0f + u) : 1.0f;
-        xv[j] = r.x.get(j);
-        gv[j] = r.g.get(j);
-        dzf[j] = 0.0f;
-        if (pz) {
-          const float z = r.z.get(j), s = sigmoid_f(z);
-          dzf[j] = gv[j] * (s * (1.0f + z * (1.0f - s)));
-          gv[j] *= z * s;
+      const int e = e0 + g * kBackCh + ch, at = (g * kBackCh + ch) * kN + kQ * q;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f), A = v;
+      if (e < E) {
+        if (p.parts > 1) {
+          v = ld4(starts + (((int64_t)b * p.parts + part) * E + e) * kN + kQ * q);
+        } else if (a.dstate_out) {
+          const float* s = a.dstate_out + ((int64_t)b * E + e) * kN + kQ * q;
+          v = make_float4(s[0], s[1], s[2], s[3]);
         }
-        sm[S::sd + row * kPitch + cl + j] = dv[j];
-        sm[S::su + row * kPitch + cl + j] = dv[j] * xv[j];
-        sm[S::sg + row * kPitch + cl + j] = gv[j];
+        const float* s = a.A + (int64_t)e * kN + kQ * q;
+        A = make_float4(s[0] * kLog2e, s[1] * kLog2e, s[2] * kLog2e, s[3] * kLog2e);
       }
-      const float4 h4 = r.h;
-      __syncthreads();
-      if (g + 1 < np) fetch(t0, g + 1);
-      else if (k > 0) fetch(t0 - kBack, 0);
-      float Av[kQ], A2[kQ], h0[kQ] = {h4.x, h4.y, h4.z, h4.w}, h[kBack][kQ], dec[kBack][kQ];
+      st4(dh_s + at, v);
+      st4(dA_s + at, make_float4(0.f, 0.f, 0.f, 0.f));
+      st4(A_s + at, A);
+    }
+    int slot = 0;
+    for (int k = tiles - 1; k >= 0; --k) {
+      const float* const bc = sm + S::bc + (k & 1) * S::kBc + kQ * q;
+      f2 vB[kBack][2], vC[kBack][2];
 #pragma unroll
-      for (int j = 0; j < kQ; ++j) {
-        Av[j] = e < E ? a.A[(int64_t)e * kN + kQ * q + j] : 0.0f;
-        A2[j] = Av[j] * kLog2e;
+      for (int t = 0; t < kBack; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vB[t][j] = vC[t][j] = f2{0ull};
+      for (int g = 0; g < np; ++g) {
+        float* const sl = sm + slot * S::kSlot;
+        const ulonglong2* const in = reinterpret_cast<const ulonglong2*>(sl) + ch;
+        const unsigned long long* const gin = reinterpret_cast<const unsigned long long*>(sl + S::gg) + ch;
+        float* const s1_s = sl + S::sums + q * kBackPitch + ch;
+        float* const s2_s = s1_s + S::kSums;
+        float* const sv_s = s2_s + S::kSums;
+        const int at = (g * kBackCh + ch) * kN + kQ * q;
+        ulonglong2 r = *reinterpret_cast<const ulonglong2*>(A_s + at);
+        const f2 A2[2] = {f2{r.x}, f2{r.y}};
+        f2 h[kBack][2], dec[kBack][2];
+        bar_sync(kFull + slot, kBackThreads);
+        r = *reinterpret_cast<const ulonglong2*>(sl + S::h0 + ch * kN + kQ * q);
+        const f2 h0[2] = {f2{r.x}, f2{r.y}};
+        float yp[4];
+#pragma unroll
+        for (int t = 0; t < kBack; ++t) {
+          r = in[t * kBackCh];
+          const f2 dd{r.x}, uu{r.y};
+          const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(bc + t * 2 * kN);
+          dec[t][0] = ex2_2(mul2(dd, A2[0]));
+          dec[t][1] = ex2_2(mul2(dd, A2[1]));
+          h[t][0] = fma2(dec[t][0], t ? h[t - 1][0] : h0[0], mul2(uu, f2{B.x}));
+          h[t][1] = fma2(dec[t][1], t ? h[t - 1][1] : h0[1], mul2(uu, f2{B.y}));
+          if (gated) {
+            const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(bc + t * 2 * kN + kN);
+            const float2 y = unpack(fma2(f2{C.x}, h[t][0], mul2(f2{C.y}, h[t][1])));
+            yp[t & 3] = y.x + y.y;
+            if ((t & 3) == 3) sv_s[(t - 3) * kBackPitch] = quad_sum(yp, q);
+          }
+        }
+        r = *reinterpret_cast<const ulonglong2*>(dh_s + at);
+        f2 dh[2] = {f2{r.x}, f2{r.y}};
+        r = *reinterpret_cast<const ulonglong2*>(dA_s + at);
+        f2 dA[2] = {f2{r.x}, f2{r.y}};
+        float p1[4], p2[4];
+#pragma unroll
+        for (int t = kBack - 1; t >= 0; --t) {
+          r = in[t * kBackCh];
+          const f2 dd{r.x}, uu{r.y}, gg{gin[t * kBackCh]};
+          const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(bc + t * 2 * kN);
+          const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(bc + t * 2 * kN + kN);
+          const f2 Bv[2] = {f2{B.x}, f2{B.y}}, Cv[2] = {f2{C.x}, f2{C.y}};
+          f2 w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) dh[j] = fma2(Cv[j], gg, dh[j]);
+          const float2 s1 = unpack(fma2(dh[0], Bv[0], mul2(dh[1], Bv[1])));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            vB[t][j] = fma2(dh[j], uu, vB[t][j]);
+            vC[t][j] = fma2(gg, h[t][j], vC[t][j]);
+            dh[j] = mul2(dh[j], dec[t][j]);
+            w[j] = mul2(dh[j], t ? h[t - 1][j] : h0[j]);
+            dA[j] = fma2(w[j], dd, dA[j]);
+          }
+          const float2 s2 = unpack(fma2(w[0], A2[0], mul2(w[1], A2[1])));
+          p1[t & 3] = s1.x + s1.y;
+          p2[t & 3] = s2.x + s2.y;
+          if ((t & 3) == 0) {
+            s1_s[t * kBackPitch] = quad_sum(p1, q);
+            s2_s[t * kBackPitch] = quad_sum(p2, q);
+          }
+        }
+        *reinterpret_cast<ulonglong2*>(dh_s + at) = make_ulonglong2(dh[0].v, dh[1].v);
+        *reinterpret_cast<ulonglong2*>(dA_s + at) = make_ulonglong2(dA[0].v, dA[1].v);
+        bar_arrive(kDone + slot, kBackThreads);
+        slot ^= 1;
       }
-      float yp[kBack];
+      // the tile's dB and dC over the warp's 8 channels: lane bits 4, 3, 0 pick C, and the state within the lane's four
+      const bool up = lane & 16, hi = lane & 8, odd = lane & 1;
+      const int t0 = begin + k * kBack;
 #pragma unroll
       for (int t = 0; t < kBack; ++t) {
-        const float d = sm[S::sd + t * kPitch + ch], du = sm[S::su + t * kPitch + ch];
-        const float4 B4 = *reinterpret_cast<const float4*>(&sm[S::sbc + t * 2 * kN + kQ * q]);
-        const float4 C4 = *reinterpret_cast<const float4*>(&sm[S::sbc + t * 2 * kN + kN + kQ * q]);
-        const float Bv[4] = {B4.x, B4.y, B4.z, B4.w}, Cv[4] = {C4.x, C4.y, C4.z, C4.w};
-        yp[t] = 0.0f;
+        const float2 b0 = unpack(vB[t][0]), b1 = unpack(vB[t][1]), c0 = unpack(vC[t][0]), c1 = unpack(vC[t][1]);
+        const float bb[4] = {b0.x, b0.y, b1.x, b1.y}, cc[4] = {c0.x, c0.y, c1.x, c1.y};
+        float k4[4];
 #pragma unroll
-        for (int j = 0; j < kQ; ++j) {
-          dec[t][j] = ex2(d * A2[j]);
-          h[t][j] = fmaf(dec[t][j], t ? h[t - 1][j] : h0[j], du * Bv[j]);
-          yp[t] = fmaf(Cv[j], h[t][j], yp[t]);
-        }
+        for (int j = 0; j < 4; ++j)
+          k4[j] = (up ? cc[j] : bb[j]) + __shfl_xor_sync(0xffffffffu, up ? bb[j] : cc[j], 16);
+        const float k0 = (hi ? k4[2] : k4[0]) + __shfl_xor_sync(0xffffffffu, hi ? k4[0] : k4[2], 8);
+        const float k1 = (hi ? k4[3] : k4[1]) + __shfl_xor_sync(0xffffffffu, hi ? k4[1] : k4[3], 8);
+        const float s = (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 1);
+        sm[S::red + (warp * kBack + t) * 2 * kN + (up ? kN : 0) + kQ * q + (hi ? 2 : 0) + (odd ? 1 : 0)] = s;
       }
-      if (pz) {
-        const float lo[4] = {yp[0], yp[1], yp[2], yp[3]}, hi[4] = {yp[4], yp[5], yp[6], yp[7]};
-        sm[S::sv + q * kPitch + ch] = quad_sum(lo, q);
-        sm[S::sv + (4 + q) * kPitch + ch] = quad_sum(hi, q);
-      }
-      float4 dh4 = *reinterpret_cast<const float4*>(dh_s + (g * kCh + ch) * kN + kQ * q);
-      float4 dA4 = *reinterpret_cast<const float4*>(dA_s + (g * kCh + ch) * kN + kQ * q);
-      float dh[4] = {dh4.x, dh4.y, dh4.z, dh4.w}, dA[4] = {dA4.x, dA4.y, dA4.z, dA4.w};
-      float p1[4], p2[4];
-#pragma unroll
-      for (int t = kBack - 1; t >= 0; --t) {
-        const float d = sm[S::sd + t * kPitch + ch], du = sm[S::su + t * kPitch + ch];
-        const float gg = sm[S::sg + t * kPitch + ch];
-        const float4 B4 = *reinterpret_cast<const float4*>(&sm[S::sbc + t * 2 * kN + kQ * q]);
-        const float4 C4 = *reinterpret_cast<const float4*>(&sm[S::sbc + t * 2 * kN + kN + kQ * q]);
-        const float Bv[4] = {B4.x, B4.y, B4.z, B4.w}, Cv[4] = {C4.x, C4.y, C4.z, C4.w};
-        float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kQ; ++j) {
-          dh[j] = fmaf(Cv[j], gg, dh[j]);
-          vB[t][j] = fmaf(dh[j], du, vB[t][j]);
-          vC[t][j] = fmaf(gg, h[t][j], vC[t][j]);
-          s1 = fmaf(dh[j], Bv[j], s1);
-          dh[j] *= dec[t][j];
-          const float w = dh[j] * (t ? h[t - 1][j] : h0[j]);
-          s2 = fmaf(w, Av[j], s2);
-          dA[j] = fmaf(w, d, dA[j]);
-        }
-        p1[t & 3] = s1;
-        p2[t & 3] = s2;
-        if ((t & 3) == 0) {
-          sm[S::s1 + (t + q) * kPitch + ch] = quad_sum(p1, q);
-          sm[S::s2 + (t + q) * kPitch + ch] = quad_sum(p2, q);
-        }
-      }
-      *reinterpret_cast<float4*>(dh_s + (g * kCh + ch) * kN + kQ * q) = make_float4(dh[0], dh[1], dh[2], dh[3]);
-      *reinterpret_cast<float4*>(dA_s + (g * kCh + ch) * kN + kQ * q) = make_float4(dA[0], dA[1], dA[2], dA[3]);
-      __syncthreads();
-      if (t0 + row < stop) {
-        float ox[2], od[2], oz[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int at = row * kPitch + cl + j;
-          const float s1 = sm[S::s1 + at];
-          ox[j] = fmaf(s1, dv[j], Dv[j] * gv[j]);
-          od[j] = in_row ? fmaf(s1, xv[j], sm[S::s2 + at]) * sig[j] : 0.0f;
-          oz[j] = pz ? dzf[j] * fmaf(Dv[j], xv[j], sm[S::sv + at]) : 0.0f;
-          float* accD = &dD_s[row * passes * kCh + g * kCh + cl + j];
-          float* accb = &db_s[row * passes * kCh + g * kCh + cl + j];
-          *accD = fmaf(gv[j], xv[j], *accD);
-          *accb += od[j];
-        }
-        const int64_t o = (orow + t0 + row) * E;
-        store_row<T, 2, VEC>((T*)a.dx + o + c, c, E, ox);
-        store_row<T, 2, VEC>((T*)a.ddt + o + c, c, E, od);
-        if (pz) store_row<T, 2, VEC>((T*)a.dz + o + c, c, E, oz);
-      }
-    }
-    // the tile's dB and dC over the warp's 8 channels: lane bits 4, 3, 2 pick C, and the state within the lane's four
-    const bool up = lane & 16, hi = lane & 8, odd = lane & 4;
-#pragma unroll
-    for (int t = 0; t < kBack; ++t) {
-      float k4[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        k4[j] = (up ? vC[t][j] : vB[t][j]) + __shfl_xor_sync(0xffffffffu, up ? vB[t][j] : vC[t][j], 16);
-      const float k0 = (hi ? k4[2] : k4[0]) + __shfl_xor_sync(0xffffffffu, hi ? k4[0] : k4[2], 8);
-      const float k1 = (hi ? k4[3] : k4[1]) + __shfl_xor_sync(0xffffffffu, hi ? k4[1] : k4[3], 8);
-      const float s = (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 4);
-      sm[S::red + (warp * kBack + t) * 2 * kN + (up ? kN : 0) + kQ * q + (hi ? 2 : 0) + (odd ? 1 : 0)] = s;
-    }
-    __syncthreads();
-    for (int i = tid; i < kBack * 2 * kN; i += kSsmThreads) {
-      const int t = t0 + i / (2 * kN);
-      if (t < stop) {
+      bar_sync(kScanOnly, kBackScan);
+      static_assert(S::kBc == kBackScan, "a thread a sum");
+      {
+        const int t = t0 + tid / (2 * kN), n = tid % (2 * kN);
         float s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) s += sm[S::red + w * kBack * 2 * kN + i];
-        bc_parts[(((int64_t)group * a.batch + b) * a.length + t) * 2 * kN + i % (2 * kN)] = s;
+        for (int w = 0; w < kBackScan / 32; ++w) s += sm[S::red + w * S::kBc + tid];
+        const int64_t rowi = (int64_t)b * a.length + t;
+        if (t < stop) {
+          if (groups > 1) bc_parts[((int64_t)group * a.batch * a.length + rowi) * 2 * kN + n] = s;
+          else if (n < kN) ((T*)a.dB)[rowi * kN + n] = from_f<T>(s);
+          else ((T*)a.dC)[rowi * kN + n - kN] = from_f<T>(s);
+        }
       }
+      bar_sync(kScanOnly, kBackScan);
     }
-  }
-  // tiles wholly behind the row's end
-  const float zero2[2] = {};
-  for (int t = begin + tiles * kBack + row; t < stop; t += kBack) {
-    const int64_t o = (orow + t) * E;
-    for (int g = 0; g < np; ++g) {
-      const int c = e0 + g * kCh + cl;
-      store_row<T, 2, VEC>((T*)a.dx + o + c, c, E, zero2);
-      store_row<T, 2, VEC>((T*)a.ddt + o + c, c, E, zero2);
-      if (pz) store_row<T, 2, VEC>((T*)a.dz + o + c, c, E, zero2);
+    __syncthreads();
+    float* const pp = param_parts + ((int64_t)b * p.parts + part) * E * (kN + 2);
+    const int channels = min(np * kBackCh, E - e0);
+    for (int i = tid; i < channels * kN; i += kBackScan) {
+      pp[(int64_t)e0 * kN + i] = dA_s[i];
+      if (part == 0 && a.dstate) a.dstate[((int64_t)b * E + e0) * kN + i] = dh_s[i];
     }
-    float* bc = bc_parts + (((int64_t)group * a.batch + b) * a.length + t) * 2 * kN + 2 * (tid & 15);
-    bc[0] = 0.0f;
-    bc[1] = 0.0f;
-  }
-  __syncthreads();
-  float* pp = param_parts + ((int64_t)b * p.parts + part) * E * (kN + 2);
-  for (int g = 0; g < np; ++g) {
-    const int e = e0 + g * kCh + ch;
-    if (e < E) {
-      const float* s = dA_s + (g * kCh + ch) * kN + kQ * q;
-      const float* d = dh_s + (g * kCh + ch) * kN + kQ * q;
-#pragma unroll
-      for (int j = 0; j < kQ; ++j) {
-        pp[(int64_t)e * kN + kQ * q + j] = s[j];
-        if (part == 0 && a.dstate) a.dstate[((int64_t)b * E + e) * kN + kQ * q + j] = d[j];
-      }
-    }
-  }
-  for (int i = tid; i < np * kCh; i += kSsmThreads) {
-    if (e0 + i < E) {
+    for (int i = tid; i < channels; i += kBackScan) {
       float sD = 0.0f, sb = 0.0f;
 #pragma unroll
       for (int k = 0; k < kBack; ++k) {
-        sD += dD_s[k * passes * kCh + i];
-        sb += db_s[k * passes * kCh + i];
+        sD += dD_s[k * width + i];
+        sb += db_s[k * width + i];
       }
       pp[(int64_t)E * kN + e0 + i] = sD;
       pp[(int64_t)E * (kN + 1) + e0 + i] = sb;
     }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kElementRegs));
+    const int tid = threadIdx.x - kBackScan;
+    const int row = tid >> 4, sub = tid & 15, cl = 4 * sub;    // four channels of token `row`; two values of its B or C
+    for (int g = 0; g < np; ++g) {
+      const int at = row * width + g * kBackCh + cl;
+      st4(dD_s + at, make_float4(0.f, 0.f, 0.f, 0.f));
+      st4(db_s + at, make_float4(0.f, 0.f, 0.f, 0.f));
+    }
+    for (int i = tid; i < np * kBackCh; i += 128) {
+      D_s[i] = a.D && e0 + i < E ? a.D[e0 + i] : 0.0f;
+      bias_s[i] = a.dt_bias && e0 + i < E ? a.dt_bias[e0 + i] : 0.0f;
+    }
+    bar_sync(kScanOnly + 1, 128);
+    const bool is_c = sub >= 8;
+    int t = begin + (tiles - 1) * kBack + row;      // of the pass to be loaded next
+    int c = e0 + cl;
+    int64_t out = ((int64_t)b * a.length + t) * E + c;   // of the pass to be finished next
+    const T* px = (const T*)a.x + b * a.x_bs + t * a.x_ts + c;
+    const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
+    const T* pz = (const T*)a.z + b * a.z_bs + t * a.z_ts + c;
+    const T* pg = (const T*)a.dy + b * a.dy_bs + t * a.dy_ts + c;
+    const T* pbc = is_c ? (const T*)a.C + b * a.C_bs + t * a.C_ts + 2 * (sub - 8)
+                        : (const T*)a.B + b * a.B_bs + t * a.B_ts + 2 * sub;
+    // states 4 (tid & 3) .. of channels tid / 4 and tid / 4 + 32 at the tile's start
+    const int nck = (a.length + kBack - 1) / kBack;
+    const float* pck = a.checkpoints + (((int64_t)b * nck + begin / kBack + tiles - 1) * E + e0) * kN + 4 * tid;
+    float4 rh[2];
+    Row<T, 4, VEC> rx, rd, rz, rg;
+    Row<T, 2, VEC> rb;
+    int g_next = 0;
+    auto fetch = [&]() {
+      const bool live = t < end;
+      rx.load(px, c, E, live);
+      rd.load(pd, c, E, live);
+      rg.load(pg, c, E, live);
+      if (gated) rz.load(pz, c, E, live);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        rh[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c - cl + (tid >> 2) + 32 * j < E) rh[j] = ld4(pck + 32 * kN * j);
+      }
+      if (g_next == 0) {
+        rb.load(pbc, 0, 2, live);
+        pbc -= kBack * (is_c ? a.C_ts : a.B_ts);
+      }
+      px += kBackCh;
+      pd += kBackCh;
+      pz += kBackCh;
+      pg += kBackCh;
+      pck += kBackCh * kN;
+      c += kBackCh;
+      if (++g_next == np) {
+        const int back = np * kBackCh;
+        g_next = 0;
+        t -= kBack;
+        c -= back;
+        px -= kBack * a.x_ts + back;
+        pd -= kBack * a.dt_ts + back;
+        pz -= kBack * a.z_ts + back;
+        pg -= kBack * a.dy_ts + back;
+        pck -= ((int64_t)E + back) * kN;
+      }
+    };
+    float ps[4], pz4[4], pxv[4], pdv[4], pgv[4];     // of the pass staged before: sigmoid, dy silu'(z), x, d, g
+    auto finish = [&](int slot, int g, bool store, bool in_row) {
+      bar_sync(kDone + slot, kBackThreads);
+      const float* const sums = sm + slot * S::kSlot + S::sums + row * kBackPitch + cl;
+      const int at = row * width + g * kBackCh + cl;
+      const float4 s1 = ld4(sums), s2 = ld4(sums + S::kSums), sv = ld4(sums + 2 * S::kSums);
+      const float4 D4 = ld4(D_s + g * kBackCh + cl), aD = ld4(dD_s + at), ab = ld4(db_s + at);
+      const float s1v[4] = {s1.x, s1.y, s1.z, s1.w}, s2v[4] = {s2.x, s2.y, s2.z, s2.w};
+      const float svv[4] = {sv.x, sv.y, sv.z, sv.w}, Dv[4] = {D4.x, D4.y, D4.z, D4.w};
+      float accD[4] = {aD.x, aD.y, aD.z, aD.w}, accb[4] = {ab.x, ab.y, ab.z, ab.w};
+      float ox[4], od[4], oz[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ox[j] = fmaf(s1v[j], pdv[j], Dv[j] * pgv[j]);
+        od[j] = in_row ? fmaf(s1v[j], pxv[j], kLn2 * s2v[j]) * ps[j] : 0.0f;   // s2 is in units of log2
+        oz[j] = gated ? pz4[j] * fmaf(Dv[j], pxv[j], svv[j]) : 0.0f;
+        accD[j] = fmaf(pgv[j], pxv[j], accD[j]);
+        accb[j] += od[j];
+      }
+      st4(dD_s + at, make_float4(accD[0], accD[1], accD[2], accD[3]));
+      st4(db_s + at, make_float4(accb[0], accb[1], accb[2], accb[3]));
+      if (store) {
+        const int oc = e0 + g * kBackCh + cl;
+        store_row<T, 4, VEC>((T*)a.dx + out, oc, E, ox);
+        store_row<T, 4, VEC>((T*)a.ddt + out, oc, E, od);
+        if (gated) store_row<T, 4, VEC>((T*)a.dz + out, oc, E, oz);
+      }
+      out += kBackCh;
+      if (g == np - 1) out -= (int64_t)kBack * E + np * kBackCh;
+    };
+    if (tiles) fetch();
+    int slot = 0;
+    bool have = false;
+    for (int k = tiles - 1; k >= 0; --k) {
+      const int ts = begin + k * kBack + row;
+      const bool in_row = ts < end;
+      for (int g = 0; g < np; ++g) {
+        const float4 b4 = ld4(bias_s + g * kBackCh + cl);
+        const float bias[4] = {b4.x, b4.y, b4.z, b4.w};
+        float sg[4], dz[4], xs[4], ds[4], gs[4];
+        float* const sl = sm + slot * S::kSlot;
+        float* const in = sl + 4 * (row * kBackCh + cl);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float raw = rd.get(j) + bias[j], x = rx.get(j);
+          float d = raw, g1 = rg.get(j);
+          sg[j] = 1.0f;
+          dz[j] = 0.0f;
+          if (a.softplus) {
+            float u;
+            d = softplus_f(raw, u);
+            sg[j] = (raw >= 0.0f ? 1.0f : u) * rcp(1.0f + u);
+          }
+          if (!in_row || e0 + g * kBackCh + cl + j >= E) d = 0.0f;
+          if (gated) {
+            const float z = rz.get(j), s = sigmoid_f(z);
+            dz[j] = g1 * (s * (1.0f + z * (1.0f - s)));
+            g1 *= z * s;
+          }
+          const float u = d * x;
+          st4(in + 4 * j, make_float4(d, d, u, u));
+          ds[j] = d;
+          gs[j] = g1;
+          xs[j] = x;
+        }
+        float* const gg = sl + S::gg + 2 * (row * kBackCh + cl);
+        st4(gg, make_float4(gs[0], gs[0], gs[1], gs[1]));
+        st4(gg + 4, make_float4(gs[2], gs[2], gs[3], gs[3]));
+        st4(sl + S::h0 + 4 * tid, rh[0]);
+        st4(sl + S::h0 + 32 * kN + 4 * tid, rh[1]);
+        if (g == 0)
+          *reinterpret_cast<float2*>(sm + S::bc + (k & 1) * S::kBc + row * 2 * kN + 2 * sub) =
+              make_float2(rb.get(0), rb.get(1));
+        bar_arrive(kFull + slot, kBackThreads);
+        if (g + 1 < np || k > 0) fetch();
+        if (have) {
+          // the pass before: of this tile, or the last of the tile behind
+          const int tp = g ? ts : ts + kBack;
+          finish(slot ^ 1, g ? g - 1 : np - 1, tp < stop, tp < end);
+        }
+        have = true;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          ps[j] = sg[j];
+          pz4[j] = dz[j];
+          pxv[j] = xs[j];
+          pdv[j] = ds[j];
+          pgv[j] = gs[j];
+        }
+        slot ^= 1;
+      }
+    }
+    if (have) finish(slot ^ 1, np - 1, begin + row < stop, begin + row < end);
+    // tiles wholly behind the row's end
+    const float zero[4] = {};
+    for (int tz = begin + tiles * kBack + row; tz < stop; tz += kBack) {
+      const int64_t rowi = (int64_t)b * a.length + tz;
+      for (int g = 0; g < np; ++g) {
+        const int oc = e0 + g * kBackCh + cl;
+        const int64_t o = rowi * E + oc;
+        store_row<T, 4, VEC>((T*)a.dx + o, oc, E, zero);
+        store_row<T, 4, VEC>((T*)a.ddt + o, oc, E, zero);
+        if (gated) store_row<T, 4, VEC>((T*)a.dz + o, oc, E, zero);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int n = 2 * sub + j;
+        if (groups > 1) bc_parts[((int64_t)group * a.batch * a.length + rowi) * 2 * kN + n] = 0.0f;
+        else if (n < kN) ((T*)a.dB)[rowi * kN + n] = from_f<T>(0.0f);
+        else ((T*)a.dC)[rowi * kN + n - kN] = from_f<T>(0.0f);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -717,15 +845,15 @@ static SsmPlan ssm_plan(const boa_ssm_args& a, int64_t row_blocks, int64_t enoug
 }
 
 static int back_passes(const boa_ssm_args& a) {
-  const int n = (a.channels + kCh - 1) / kCh;
+  const int n = (a.channels + kBackCh - 1) / kBackCh;
   return n < kPasses ? n : kPasses;
 }
 static int back_groups(const boa_ssm_args& a) {
-  const int per = back_passes(a) * kCh;
+  const int per = back_passes(a) * kBackCh;
   return (a.channels + per - 1) / per;
 }
 static SsmPlan plan_forward(const boa_ssm_args& a) { return ssm_plan(a, (a.channels + kCh - 1) / kCh, 888, 1776); }
-static SsmPlan plan_backward(const boa_ssm_args& a) { return ssm_plan(a, back_groups(a), 444, 1776); }
+static SsmPlan plan_backward(const boa_ssm_args& a) { return ssm_plan(a, back_groups(a), 444, 592); }
 
 // Vector accesses where every row of every tensor starts on four elements.
 static bool row_vec(const void* p, int64_t bs, int64_t ts, size_t size) {
@@ -770,7 +898,7 @@ static int ssm_backward_t(const boa_ssm_args& a, cudaStream_t s) {
   const SsmPlan p = plan_backward(a);
   const int passes = back_passes(a), groups = back_groups(a);
   float* bc = (float*)a.workspace;
-  float* params = bc + (size_t)groups * a.batch * a.length * 2 * kN;
+  float* params = bc + (groups > 1 ? (size_t)groups * a.batch * a.length * 2 * kN : 0);
   float* ends = params + (size_t)a.batch * p.parts * a.channels * (kN + 2);
   // the three sections keep 16-byte alignment: ends holds float4
   ends = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ends) + 15) & ~uintptr_t(15));
@@ -782,11 +910,16 @@ static int ssm_backward_t(const boa_ssm_args& a, cudaStream_t s) {
     k_ssm_join<<<(unsigned)((n + 127) / 128), 128, 0, s>>>(n, a.channels, p.parts, a.A, a.dstate_out, ends, dsum, true);
   }
   const int smem = BackSmem::floats(passes) * (int)sizeof(float);
+  // setmaxnreg moves registers between the two warpgroups: the launch has to hold exactly their sum
+  cudaFuncAttributes fa{};
+  BOA_CUDA(cudaFuncGetAttributes(&fa, k_ssm_backward<T, VEC>));
+  if (fa.numRegs != kBackRegs)
+    return boa_fail(BOA_ERR_UNSUPPORTED, "boa_ssm_scan_backward: built with another register count than its split");
   BOA_CUDA(cudaFuncSetAttribute(k_ssm_backward<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  k_ssm_backward<T, VEC><<<(unsigned)((int64_t)groups * p.parts * a.batch), kSsmThreads, smem, s>>>(a, p, passes, groups,
+  k_ssm_backward<T, VEC><<<(unsigned)((int64_t)groups * p.parts * a.batch), kBackThreads, smem, s>>>(a, p, passes, groups,
                                                                                              ends, bc, params);
   const int64_t rows = (int64_t)a.batch * a.length, n = rows * 2 * kN;
-  if (n > 0)
+  if (n > 0 && groups > 1)
     k_ssm_bc<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(rows, groups, bc, (T*)a.dB, (T*)a.dC);
   const int cols = a.channels * (kN + 2);
   k_sum_parts<<<(cols + 31) / 32, 512, 0, s>>>(params, (int64_t)a.batch * p.parts, cols, a.channels * kN,
@@ -826,7 +959,8 @@ BOA_API size_t boa_ssm_workspace_bytes(const boa_ssm_args* a, int backward) {
   if (ssm_check(a, "boa_ssm_workspace_bytes") || a->batch == 0) return 0;
   if (!backward) return ends_floats(*a, plan_forward(*a)) * sizeof(float);
   const SsmPlan p = plan_backward(*a);
-  return (ends_floats(*a, p) + (size_t)back_groups(*a) * a->batch * a->length * 2 * kN +
+  const size_t groups = back_groups(*a);
+  return (ends_floats(*a, p) + (groups > 1 ? groups * a->batch * a->length * 2 * kN : 0) +
           (size_t)a->batch * p.parts * a->channels * (kN + 2)) * sizeof(float) + 16;
 }
 
