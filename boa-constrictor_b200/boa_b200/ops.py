@@ -41,6 +41,8 @@ _DTYPES = {torch.float32: _n.BOA_DTYPE_F32, torch.bfloat16: _n.BOA_DTYPE_BF16, t
 
 
 # ------------------------------------------------------------------ arguments
+# The host side of a one-token call is most of its time, so the checks compare
+# shapes and device indexes directly and the library's functions are looked up once.
 def _kind(who, x):
     k = _DTYPES.get(x.dtype)
     if k is None:
@@ -49,23 +51,25 @@ def _kind(who, x):
 
 
 def _shape(who, name, t, shape):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{who}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _same(who, x, **others):
+def _same(who, x, name, t):
     """Activations of one call share x's type."""
-    for name, t in others.items():
-        if t is not None and t.dtype != x.dtype:
-            raise ValueError(f"{who}: {name} must have the type of x ({x.dtype}), got {t.dtype}")
+    if t.dtype != x.dtype:
+        raise ValueError(f"{who}: {name} must have the type of x ({x.dtype}), got {t.dtype}")
 
 
 def _on_device(who, x, *others):
-    if not x.is_cuda:
+    """The index of the CUDA device that holds every tensor."""
+    index = x.get_device()
+    if index < 0:
         raise RuntimeError(f"{who} runs on CUDA devices only (no CPU path)")
     for t in others:
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != index:
             raise RuntimeError(f"{who}: all tensors must be on {x.device}, got one on {t.device}")
+    return index
 
 
 def _param(t):
@@ -100,30 +104,48 @@ def _ptr(t):
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _call(name, device, *args):
-    """One library call on the device's current stream."""
-    stream = ctypes.c_void_p(_n.stream_ptr(device))
-    if torch.cuda.current_device() == device.index:
-        _n.call(name, *args, stream)
+_functions = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _n.stream_ptr)   # handle of the device's current stream
+
+
+def _fn(name):
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(_n.load(), name)
+    return f
+
+
+def _call(name, index, *args):
+    """One library call on device `index`'s current stream."""
+    f = _functions.get(name) or _fn(name)
+    if torch.cuda.current_device() == index:
+        rc = f(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            _n.call(name, *args, stream)
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
+    if rc:
+        _n.check(rc, name)
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _workspace(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 # ----------------------------------------------------------------- layer norm
 def _norm_forward(x, weight, bias, eps, keep_stats):
     rows, width = x.shape
-    y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep_stats else None
-    _call("boa_layer_norm", x.device, rows, width, _DTYPES[x.dtype], _ptr(x), x.stride(0), _ptr(weight), _ptr(bias),
-          eps, _ptr(y), _ptr(stats), x.device.index)
+    y = x.new_empty((rows, width))
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if keep_stats else None
+    index = x.get_device()
+    _call("boa_layer_norm", index, rows, width, _DTYPES[x.dtype], x.data_ptr(), x.stride(0), weight.data_ptr(),
+          _ptr(bias), eps, y.data_ptr(), _ptr(stats), index)
     return y, stats
 
 
@@ -141,14 +163,15 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, stats = ctx.saved_tensors
         rows, width = x.shape
         dy = _rows(dy)
-        dx = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        dx = x.new_empty((rows, width))
         dw = torch.empty_like(weight)
         db = torch.empty_like(weight) if ctx.with_bias else None
-        kind = _DTYPES[x.dtype]
-        nbytes = _n.load().boa_layer_norm_workspace_bytes(rows, width, kind)
-        ws = _workspace(nbytes, x.device)
-        _call("boa_layer_norm_backward", x.device, rows, width, kind, _ptr(x), x.stride(0), _ptr(dy), dy.stride(0),
-              _ptr(weight), _ptr(stats), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, x.device.index)
+        kind, index = _DTYPES[x.dtype], x.get_device()
+        nbytes = _fn("boa_layer_norm_workspace_bytes")(rows, width, kind)
+        ws = _workspace(nbytes, x)
+        _call("boa_layer_norm_backward", index, rows, width, kind, x.data_ptr(), x.stride(0), dy.data_ptr(),
+              dy.stride(0), weight.data_ptr(), stats.data_ptr(), dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(ws),
+              nbytes, index)
         return dx, dw, db, None
 
 
@@ -157,41 +180,38 @@ def layer_norm(x, weight, bias=None, eps: float = 1e-5):
     (1 to 8192 wide); weight and bias are ``[width]``."""
     who = "layer_norm"
     _kind(who, x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{who}: x needs a last axis of at least one element, got shape {tuple(x.shape)}")
-    width = x.shape[-1]
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{who}: x needs a last axis of at least one element, got shape {tuple(shape)}")
+    width = shape[-1]
     _shape(who, "weight", weight, (width,))
     if bias is not None:
         _shape(who, "bias", bias, (width,))
     _on_device(who, x, weight, bias)
     weight, bias = _param(weight), _param(bias)
-    flat = _rows(x.reshape(-1, width))
+    flat = _rows(x if len(shape) == 2 else x.reshape(-1, width))
     if _wants_grad(x, weight, bias):
         y = _LayerNorm.apply(flat, weight, bias, float(eps))
     else:
         y, _ = _norm_forward(flat, weight, bias, float(eps), False)
-    return y.view(x.shape)
+    return y if len(shape) == 2 else y.view(shape)
 
 
 # --------------------------------------------------------- causal convolution
-def _conv_args(x, weight, bias, silu, state, lens):
-    a = _n.ConvArgs()
-    a.dtype, a.batch, a.channels, a.width = _DTYPES[x.dtype], x.shape[0], x.shape[-1], weight.shape[1]
-    a.silu, a.device = int(silu), x.device.index
-    a.x, a.x_bs = _ptr(x), x.stride(0)
-    if x.dim() == 3:
-        a.length, a.x_ts = x.shape[1], x.stride(1)
-    a.weight, a.bias, a.state, a.lens = _ptr(weight), _ptr(bias), _ptr(state), _ptr(lens)
-    return a
+def _conv_args(x, weight, bias, silu, state, lens, y=None, state_out=None):
+    shape, strides = x.shape, x.stride()
+    step = len(shape) == 2
+    return _n.ConvArgs(_DTYPES[x.dtype], shape[0], 0 if step else shape[1], shape[-1], weight.shape[1], int(silu),
+                       x.get_device(), 0, x.data_ptr(), strides[0], 0 if step else strides[1], weight.data_ptr(),
+                       _ptr(bias), _ptr(state), _ptr(lens), _ptr(y), _ptr(state_out))
 
 
 def _conv_forward(x, weight, bias, silu, state, lens, return_state):
-    a = _conv_args(x, weight, bias, silu, state, lens)
     b, length, e = x.shape
-    y = torch.empty((b, length, e), dtype=x.dtype, device=x.device)
-    out = torch.empty((b, a.width - 1, e), dtype=x.dtype, device=x.device) if return_state else None
-    a.y, a.state_out = _ptr(y), _ptr(out)
-    _call("boa_causal_conv", x.device, ctypes.byref(a))
+    y = x.new_empty((b, length, e))
+    out = x.new_empty((b, weight.shape[1] - 1, e)) if return_state else None
+    a = _conv_args(x, weight, bias, silu, state, lens, y, out)
+    _call("boa_causal_conv", a.device, ctypes.byref(a))
     return y, out
 
 
@@ -209,18 +229,18 @@ class _CausalConv(torch.autograd.Function):
     def backward(ctx, dy, dout):
         x, weight, bias, state, lens = ctx.saved_tensors
         a = _conv_args(x, weight, bias, ctx.silu, state, lens)
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _rows(dy)
+        dy = x.new_zeros(x.shape) if dy is None else _rows(dy)
         dout = None if dout is None else dout.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = x.new_empty(x.shape)
         dw = torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         ds = None if state is None else torch.empty_like(state)
         a.dy, a.dy_bs, a.dy_ts, a.dstate_out = _ptr(dy), dy.stride(0), dy.stride(1), _ptr(dout)
         a.dx, a.dweight, a.dbias, a.dstate = _ptr(dx), _ptr(dw), _ptr(db), _ptr(ds)
-        a.workspace_bytes = _n.load().boa_causal_conv_workspace_bytes(ctypes.byref(a))
-        ws = _workspace(a.workspace_bytes, x.device)
+        a.workspace_bytes = _fn("boa_causal_conv_workspace_bytes")(ctypes.byref(a))
+        ws = _workspace(a.workspace_bytes, x)
         a.workspace = _ptr(ws)
-        _call("boa_causal_conv_backward", x.device, ctypes.byref(a))
+        _call("boa_causal_conv_backward", a.device, ctypes.byref(a))
         return dx, dw, db, ds, None, None, None
 
 
@@ -251,7 +271,7 @@ def causal_conv(x, weight, bias=None, *, silu: bool = True, state=None, lens=Non
         _shape(who, "bias", bias, (e,))
     if state is not None:
         _shape(who, "state", state, (b, weight.shape[1] - 1, e))
-    _same(who, x, state=state)
+        _same(who, x, "state", state)
     lens = _lens(who, lens, b, length)
     _on_device(who, x, weight, bias, state, lens)
     weight, bias, x = _param(weight), _param(bias), _rows(x)
@@ -275,49 +295,47 @@ def causal_conv_step(x, state, weight, bias=None, *, silu: bool = True):
     if bias is not None:
         _shape(who, "bias", bias, (x.shape[1],))
     _shape(who, "state", state, (x.shape[0], weight.shape[1] - 1, x.shape[1]))
-    _same(who, x, state=state)
+    _same(who, x, "state", state)
     if not state.is_contiguous():
         raise ValueError(f"{who}: state is updated in place and must be contiguous")
     _on_device(who, x, state, weight, bias)
     if _wants_grad(x, state, weight, bias):
         raise RuntimeError(f"{who} has no gradient: call it under torch.no_grad(), or use causal_conv")
     weight, bias, x = _param(weight), _param(bias), _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _conv_args(x, weight, bias, silu, None, None)
-    a.y, a.state_out = _ptr(y), _ptr(state)
-    _call("boa_causal_conv_step", x.device, ctypes.byref(a))
+    y = x.new_empty(x.shape)
+    a = _conv_args(x, weight, bias, silu, None, None, y, state)
+    _call("boa_causal_conv_step", a.device, ctypes.byref(a))
     return y
 
 
 # ----------------------------------------------------- selective state space scan
-def _ssm_args(x, dt, A, B, C, D, z, dt_bias, softplus, state, lens):
-    a = _n.SsmArgs()
-    a.dtype, a.batch, a.channels, a.states = _DTYPES[x.dtype], x.shape[0], x.shape[-1], A.shape[1]
-    a.softplus, a.device = int(softplus), x.device.index
-    a.x, a.dt, a.B, a.C, a.z = _ptr(x), _ptr(dt), _ptr(B), _ptr(C), _ptr(z)
-    a.x_bs, a.dt_bs, a.B_bs, a.C_bs = x.stride(0), dt.stride(0), B.stride(0), C.stride(0)
-    if z is not None:
-        a.z_bs = z.stride(0)
-    if x.dim() == 3:
-        a.length = x.shape[1]
-        a.x_ts, a.dt_ts, a.B_ts, a.C_ts = x.stride(1), dt.stride(1), B.stride(1), C.stride(1)
-        if z is not None:
-            a.z_ts = z.stride(1)
-    a.A, a.D, a.dt_bias, a.state, a.lens = _ptr(A), _ptr(D), _ptr(dt_bias), _ptr(state), _ptr(lens)
-    return a
+def _ssm_args(x, dt, A, B, C, D, z, dt_bias, softplus, state, lens, y=None, state_out=None, checkpoints=None):
+    shape = x.shape
+    if len(shape) == 2:
+        length, xs, ds, Bs, Cs = 0, (x.stride(0), 0), (dt.stride(0), 0), (B.stride(0), 0), (C.stride(0), 0)
+        zs = (0, 0) if z is None else (z.stride(0), 0)
+    else:
+        length, xs, ds, Bs, Cs = shape[1], x.stride(), dt.stride(), B.stride(), C.stride()
+        zs = (0, 0) if z is None else z.stride()
+    return _n.SsmArgs(_DTYPES[x.dtype], shape[0], length, shape[-1], D_STATE, int(softplus), x.get_device(), 0,
+                      x.data_ptr(), dt.data_ptr(), _ptr(z), B.data_ptr(), C.data_ptr(),
+                      xs[0], xs[1], ds[0], ds[1], zs[0], zs[1], Bs[0], Bs[1], Cs[0], Cs[1],
+                      A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(state), _ptr(lens), _ptr(y), _ptr(state_out),
+                      _ptr(checkpoints))
 
 
 def _ssm_forward(x, dt, A, B, C, D, z, dt_bias, softplus, state, lens, return_state, keep):
-    a = _ssm_args(x, dt, A, B, C, D, z, dt_bias, softplus, state, lens)
-    lib = _n.load()
     b, length, e = x.shape
-    y = torch.empty((b, length, e), dtype=x.dtype, device=x.device)
-    out = torch.empty((b, e, D_STATE), dtype=torch.float32, device=x.device) if return_state else None
-    checkpoints = _workspace(lib.boa_ssm_checkpoint_bytes(ctypes.byref(a)), x.device) if keep else None
-    a.workspace_bytes = lib.boa_ssm_workspace_bytes(ctypes.byref(a), 0)
-    ws = _workspace(a.workspace_bytes, x.device)
-    a.y, a.state_out, a.checkpoints, a.workspace = _ptr(y), _ptr(out), _ptr(checkpoints), _ptr(ws)
-    _call("boa_ssm_scan", x.device, ctypes.byref(a))
+    y = x.new_empty((b, length, e))
+    out = A.new_empty((b, e, D_STATE)) if return_state else None
+    a = _ssm_args(x, dt, A, B, C, D, z, dt_bias, softplus, state, lens, y, out)
+    r = ctypes.byref(a)
+    checkpoints = _workspace(_fn("boa_ssm_checkpoint_bytes")(r), x) if keep else None
+    a.checkpoints = _ptr(checkpoints)
+    a.workspace_bytes = _fn("boa_ssm_workspace_bytes")(r, 0)
+    ws = _workspace(a.workspace_bytes, x)
+    a.workspace = _ptr(ws)
+    _call("boa_ssm_scan", a.device, r)
     return y, out, checkpoints
 
 
@@ -334,38 +352,42 @@ class _SsmScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dout):
         x, dt, A, B, C, D, z, dt_bias, state, lens, checkpoints = ctx.saved_tensors
-        a = _ssm_args(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, state, lens)
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _rows(dy)
+        a = _ssm_args(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, state, lens, checkpoints=checkpoints)
+        dy = x.new_zeros(x.shape) if dy is None else _rows(dy)
         dout = None if dout is None else dout.contiguous()
-        fresh = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        fresh = lambda t: None if t is None else t.new_empty(t.shape)  # noqa: E731
         dx, ddt, dA, dB, dC, dD, dz, dbias, ds = (fresh(t) for t in (x, dt, A, B, C, D, z, dt_bias, state))
         a.dy, a.dy_bs, a.dy_ts, a.dstate_out = _ptr(dy), dy.stride(0), dy.stride(1), _ptr(dout)
-        a.checkpoints = _ptr(checkpoints)
         a.dx, a.ddt, a.dA, a.dB, a.dC = _ptr(dx), _ptr(ddt), _ptr(dA), _ptr(dB), _ptr(dC)
         a.dD, a.dz, a.ddt_bias, a.dstate = _ptr(dD), _ptr(dz), _ptr(dbias), _ptr(ds)
-        a.workspace_bytes = _n.load().boa_ssm_workspace_bytes(ctypes.byref(a), 1)
-        ws = _workspace(a.workspace_bytes, x.device)
+        r = ctypes.byref(a)
+        a.workspace_bytes = _fn("boa_ssm_workspace_bytes")(r, 1)
+        ws = _workspace(a.workspace_bytes, x)
         a.workspace = _ptr(ws)
-        _call("boa_ssm_scan_backward", x.device, ctypes.byref(a))
+        _call("boa_ssm_scan_backward", a.device, r)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, ds, None, None, None
 
 
 def _ssm_check(who, x, dt, A, B, C, D, z, dt_bias, dims):
     _kind(who, x)
-    if x.dim() != dims or x.shape[-1] < 1:
-        raise ValueError(f"{who}: x must be [batch, {'length, ' if dims == 3 else ''}channels], got {tuple(x.shape)}")
-    e, at = x.shape[-1], tuple(x.shape[:-1])
-    _shape(who, "dt", dt, x.shape)
-    if A.dim() != 2 or tuple(A.shape) != (e, D_STATE):
-        raise ValueError(f"{who}: A must be [{e}, {D_STATE}], got {tuple(A.shape)}")
-    _shape(who, "B", B, at + (D_STATE,))
-    _shape(who, "C", C, at + (D_STATE,))
-    for name, t in (("D", D), ("dt_bias", dt_bias)):
-        if t is not None:
-            _shape(who, name, t, (e,))
+    shape = x.shape
+    if len(shape) != dims or shape[-1] < 1:
+        raise ValueError(f"{who}: x must be [batch, {'length, ' if dims == 3 else ''}channels], got {tuple(shape)}")
+    e, bc = shape[-1], (*shape[:-1], D_STATE)
+    _shape(who, "dt", dt, shape)
+    _shape(who, "A", A, (e, D_STATE))
+    _shape(who, "B", B, bc)
+    _shape(who, "C", C, bc)
+    if D is not None:
+        _shape(who, "D", D, (e,))
+    if dt_bias is not None:
+        _shape(who, "dt_bias", dt_bias, (e,))
     if z is not None:
-        _shape(who, "z", z, x.shape)
-    _same(who, x, dt=dt, B=B, C=C, z=z)
+        _shape(who, "z", z, shape)
+        _same(who, x, "z", z)
+    _same(who, x, "dt", dt)
+    _same(who, x, "B", B)
+    _same(who, x, "C", C)
 
 
 def _state32(who, state, x):
@@ -414,8 +436,7 @@ def ssm_step(x, dt, state, A, B, C, D=None, z=None, dt_bias=None, *, softplus: b
         raise RuntimeError(f"{who} has no gradient: call it under torch.no_grad(), or use ssm_scan")
     A, D, dt_bias = _param(A), _param(D), _param(dt_bias)
     x, dt, B, C, z = _rows(x), _rows(dt), _rows(B), _rows(C), _rows(z)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _ssm_args(x, dt, A, B, C, D, z, dt_bias, softplus, None, None)
-    a.y, a.state_out = _ptr(y), _ptr(state)
-    _call("boa_ssm_step", x.device, ctypes.byref(a))
+    y = x.new_empty(x.shape)
+    a = _ssm_args(x, dt, A, B, C, D, z, dt_bias, softplus, None, None, y, state)
+    _call("boa_ssm_step", a.device, ctypes.byref(a))
     return y

@@ -31,22 +31,39 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
-// VPL values of a row per thread, as VPL / V accesses of V elements.
+// VPL values of a row per thread, as VPL / V accesses of V elements, zeros
+// beyond the width.
 template <typename T, int V, int VPL, int ROW_WARPS>
-__device__ __forceinline__ void row_load(const T* row, int width, int lane, float (&v)[VPL]) {
+struct NormRow {
+  Words<T, V> r[VPL / V];
+  __device__ __forceinline__ void load(const T* row, int width, int lane) {
 #pragma unroll
-  for (int c = 0; c < VPL / V; ++c) {
-    const int i = (c * 32 * ROW_WARPS + lane) * V;
-    float t[V];
-    if (i < width) {
-      load_f<T, V>(row + i, t);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) t[j] = 0.0f;
+    for (int c = 0; c < VPL / V; ++c) {
+      const int i = (c * 32 * ROW_WARPS + lane) * V;
+      r[c].clear();
+      if (i < width) r[c].load(row + i);
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[c * V + j] = t[j];
   }
+  __device__ __forceinline__ void get(float (&v)[VPL]) const {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) v[i] = r[i / V].get(i % V);
+  }
+};
+
+// Rows a warp works on together: their loads and reductions overlap.
+template <int VPL, int ROW_WARPS>
+constexpr int norm_rows() { return ROW_WARPS > 1 ? 1 : VPL <= 8 ? 4 : VPL <= 16 ? 2 : 1; }
+
+// A column's parameters in registers, zeros beyond the width or without the array.
+template <int V, int VPL, int ROW_WARPS>
+__device__ __forceinline__ void param_load(const float* p, int width, int lane, float (&v)[VPL]) {
+#pragma unroll
+  for (int c = 0; c < VPL / V; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int i = (c * 32 * ROW_WARPS + lane) * V + j;
+      v[c * V + j] = p && i < width ? p[i] : 0.0f;
+    }
 }
 
 template <typename T, int V, int VPL, int ROW_WARPS>
@@ -55,41 +72,61 @@ __global__ void __launch_bounds__(kNormWarps * 32) k_norm(int64_t rows, int widt
                                                           const float* __restrict__ b, float eps, T* __restrict__ y,
                                                           float* __restrict__ stats) {
   __shared__ float red[ROW_WARPS];
-  constexpr int kLanes = 32 * ROW_WARPS;
-  constexpr int kRows = kNormWarps / ROW_WARPS;
+  constexpr int kLanes = 32 * ROW_WARPS, R = norm_rows<VPL, ROW_WARPS>();
+  constexpr int kRows = kNormWarps / ROW_WARPS * R;
   const int lane = threadIdx.x % kLanes;
   const float inv = 1.0f / (float)width;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; row < rows; row += (int64_t)gridDim.x * kRows) {
-    float v[VPL];
-    row_load<T, V, VPL, ROW_WARPS>(x + row * x_stride, width, lane, v);
-    float s = 0.0f;
+  float wv[VPL], bv[VPL];
+  param_load<V, VPL, ROW_WARPS>(w, width, lane, wv);
+  param_load<V, VPL, ROW_WARPS>(b, width, lane, bv);
+  NormRow<T, V, VPL, ROW_WARPS> next[R];      // the rows of the next round are in flight while these are worked on
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) s += v[i];
-    const float mean = row_sum<ROW_WARPS>(s, red) * inv;
-    float q = 0.0f;
+    for (int k = 0; k < R; ++k) next[k].load(x + min(row + k, rows - 1) * x_stride, width, lane);
+  };
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes * R;
+  if (row < rows) fetch(row);
+  for (; row < rows; row += (int64_t)gridDim.x * kRows) {
+    float v[R][VPL], s[R], mean[R], rstd[R];
 #pragma unroll
-    for (int c = 0; c < VPL / V; ++c)
+    for (int k = 0; k < R; ++k) next[k].get(v[k]);
+    if (row + (int64_t)gridDim.x * kRows < rows) fetch(row + (int64_t)gridDim.x * kRows);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[c * V + j] - mean;
-        q += ((c * kLanes + lane) * V < width) ? d * d : 0.0f;
-      }
-    const float rstd = rsqrtf(row_sum<ROW_WARPS>(q, red) * inv + eps);
-    if (stats && lane == 0) {
-      stats[2 * row] = mean;
-      stats[2 * row + 1] = rstd;
+    for (int k = 0; k < R; ++k) {
+      s[k] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) s[k] += v[k][i];
     }
 #pragma unroll
-    for (int c = 0; c < VPL / V; ++c) {
-      const int i = (c * kLanes + lane) * V;
-      if (i < width) {
-        float o[V];
+    for (int k = 0; k < R; ++k) mean[k] = row_sum<ROW_WARPS>(s[k], red) * inv;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      s[k] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < VPL / V; ++c)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          o[j] = (v[c * V + j] - mean) * rstd * w[i + j];
-          if (b) o[j] += b[i + j];
+          v[k][c * V + j] -= mean[k];
+          const float d = v[k][c * V + j];
+          s[k] += ((c * kLanes + lane) * V < width) ? d * d : 0.0f;
         }
-        store_f<T, V>(y + row * width + i, o);
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) rstd[k] = rsqrtf(row_sum<ROW_WARPS>(s[k], red) * inv + eps);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (row + k >= rows) break;
+      if (stats && lane == 0)
+        *reinterpret_cast<float2*>(stats + 2 * (row + k)) = make_float2(mean[k], rstd[k]);
+#pragma unroll
+      for (int c = 0; c < VPL / V; ++c) {
+        const int i = (c * kLanes + lane) * V;
+        if (i < width) {
+          float o[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j] = fmaf(v[k][c * V + j] * rstd[k], wv[c * V + j], bv[c * V + j]);
+          store_f<T, V>(y + (row + k) * width + i, o);
+        }
       }
     }
   }
@@ -105,49 +142,73 @@ __global__ void __launch_bounds__(kNormWarps * 32)
                     T* __restrict__ dx, float* __restrict__ parts) {
   extern __shared__ float joined[];   // [2 * width]
   __shared__ float red[ROW_WARPS];
-  constexpr int kLanes = 32 * ROW_WARPS;
-  constexpr int kRows = kNormWarps / ROW_WARPS;
+  constexpr int kLanes = 32 * ROW_WARPS, R = norm_rows<VPL, ROW_WARPS>() > 1 ? 2 : 1;
+  constexpr int kSubs = kNormWarps / ROW_WARPS, kRows = kSubs * R;
   const int lane = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
   const float inv = 1.0f / (float)width;
   float wv[VPL], dw[VPL], db[VPL];
+  param_load<V, VPL, ROW_WARPS>(w, width, lane, wv);
 #pragma unroll
-  for (int c = 0; c < VPL / V; ++c)
+  for (int i = 0; i < VPL; ++i) dw[i] = db[i] = 0.0f;
+  NormRow<T, V, VPL, ROW_WARPS> nx[R], ng[R];      // the next round's rows, in flight
+  float2 nst[R];
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int i = (c * kLanes + lane) * V + j;
-      wv[c * V + j] = i < width ? w[i] : 0.0f;
-      dw[c * V + j] = 0.0f;
-      db[c * V + j] = 0.0f;
+    for (int k = 0; k < R; ++k) {
+      const int64_t r = min(row + k, rows - 1);
+      nx[k].load(x + r * x_stride, width, lane);
+      ng[k].load(dy + r * dy_stride, row + k < rows ? width : 0, lane);   // a row past the last: dy counts as zero
+      nst[k] = *reinterpret_cast<const float2*>(stats + 2 * r);
     }
-  for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < rows; row += (int64_t)gridDim.x * kRows) {
-    float xv[VPL], gv[VPL];
-    row_load<T, V, VPL, ROW_WARPS>(x + row * x_stride, width, lane, xv);
-    row_load<T, V, VPL, ROW_WARPS>(dy + row * dy_stride, width, lane, gv);
-    const float mean = stats[2 * row], rstd = stats[2 * row + 1];
-    float s = 0.0f, q = 0.0f;
+  };
+  int64_t row = (int64_t)blockIdx.x * kRows + sub * R;
+  if (row < rows) fetch(row);
+  for (; row < rows; row += (int64_t)gridDim.x * kRows) {
+    float xv[R][VPL], gv[R][VPL], s[R], q[R], rstd[R];
+    float2 stv[R];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      xv[i] = (xv[i] - mean) * rstd;
-      dw[i] += gv[i] * xv[i];      // dy is 0 beyond the width
-      db[i] += gv[i];
-      gv[i] *= wv[i];
-      s += gv[i];
-      q += gv[i] * xv[i];
+    for (int k = 0; k < R; ++k) {
+      nx[k].get(xv[k]);
+      ng[k].get(gv[k]);
+      stv[k] = nst[k];
     }
-    s = row_sum<ROW_WARPS>(s, red) * inv;
-    q = row_sum<ROW_WARPS>(q, red) * inv;
+    if (row + (int64_t)gridDim.x * kRows < rows) fetch(row + (int64_t)gridDim.x * kRows);
 #pragma unroll
-    for (int c = 0; c < VPL / V; ++c) {
-      const int i = (c * kLanes + lane) * V;
-      if (i < width) {
-        float o[V];
+    for (int k = 0; k < R; ++k) {
+      const float2 st = stv[k];
+      rstd[k] = st.y;
+      s[k] = q[k] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = rstd * (gv[c * V + j] - s - xv[c * V + j] * q);
-        store_f<T, V>(dx + row * width + i, o);
+      for (int i = 0; i < VPL; ++i) {
+        xv[k][i] = (xv[k][i] - st.x) * st.y;
+        dw[i] = fmaf(gv[k][i], xv[k][i], dw[i]);      // dy is 0 beyond the width
+        db[i] += gv[k][i];
+        gv[k][i] *= wv[i];
+        s[k] += gv[k][i];
+        q[k] = fmaf(gv[k][i], xv[k][i], q[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      s[k] = row_sum<ROW_WARPS>(s[k], red) * inv;
+      q[k] = row_sum<ROW_WARPS>(q[k], red) * inv;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (row + k >= rows) break;
+#pragma unroll
+      for (int c = 0; c < VPL / V; ++c) {
+        const int i = (c * kLanes + lane) * V;
+        if (i < width) {
+          float o[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j] = rstd[k] * (gv[k][c * V + j] - s[k] - xv[k][c * V + j] * q[k]);
+          store_f<T, V>(dx + (row + k) * width + i, o);
+        }
       }
     }
   }
-  for (int k = 0; k < kRows; ++k) {
+  for (int k = 0; k < kSubs; ++k) {
     if (sub == k) {
 #pragma unroll
       for (int c = 0; c < VPL / V; ++c)
@@ -182,9 +243,9 @@ struct NormCall {
 };
 
 // Blocks of the backward kernel (its workspace holds a row of sums per block):
-// 4 blocks on every SM of the largest B200 part, fewer when the rows are few.
+// 4 blocks on every one of 148 SMs, fewer when the rows are few.
 static int norm_backward_grid(int64_t rows, int width) {
-  const int64_t per = width <= 1024 ? kNormWarps : 1;
+  const int64_t per = width <= 512 ? 2 * kNormWarps : width <= 1024 ? kNormWarps : 1;
   const int64_t need = (rows + per - 1) / per;
   return (int)(need < 592 ? need : 592);
 }
@@ -259,7 +320,7 @@ BOA_API int boa_layer_norm(int64_t rows, int width, int dtype, const void* d_x, 
   NormCall c{};
   c.rows = rows; c.width = width; c.dtype = dtype; c.x = d_x; c.x_stride = x_stride;
   c.w = d_weight; c.b = d_bias; c.eps = eps; c.out = d_y; c.stats = d_stats; c.s = (cudaStream_t)stream;
-  const int64_t per = width <= 1024 ? kNormWarps : 1;
+  const int64_t per = width <= 256 ? 4 * kNormWarps : width <= 512 ? 2 * kNormWarps : width <= 1024 ? kNormWarps : 1;
   const int64_t need = (rows + per - 1) / per, most = (int64_t)n_sms(device) * 8;
   c.grid = (int)(need < most ? need : most);
   return norm_dispatch(c, false);

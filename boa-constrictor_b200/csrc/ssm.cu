@@ -17,8 +17,6 @@
 // taken.  The backward call does the same with the gradient of the state, in
 // reverse, and restarts h from checkpoints every 8 tokens that the forward call
 // leaves.
-#include <cstring>
-
 #include "seq_common.cuh"
 
 namespace boa {
@@ -43,44 +41,14 @@ __device__ __forceinline__ int row_len(const boa_ssm_args& a, int b) {
 // values are used a tile later.
 template <typename T, int V, bool VEC>
 struct Row {
-  static constexpr int kWords = VEC ? V * (int)sizeof(T) / 4 : V;
-  uint32_t w[kWords];
-  __device__ __forceinline__ float get(int j) const {
-    if constexpr (sizeof(T) == 4) {
-      return __uint_as_float(w[j]);
-    } else {
-      const unsigned short h = VEC ? (unsigned short)(w[j / 2] >> (16 * (j & 1))) : (unsigned short)w[j];
-      T t;
-      memcpy(&t, &h, 2);
-      return to_f(t);
-    }
-  }
+  static constexpr int kVecs = VEC ? 1 : V;
+  Words<T, VEC ? V : 1> v[kVecs];
+  __device__ __forceinline__ float get(int j) const { return VEC ? v[0].get(j) : v[VEC ? 0 : j].get(0); }
   __device__ __forceinline__ void load(const T* p, int c, int E, bool live) {
 #pragma unroll
-    for (int j = 0; j < kWords; ++j) w[j] = 0;
-    if constexpr (VEC) {
-      if (live && c < E) {
-        if constexpr (kWords == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
-        if constexpr (kWords == 2) {
-          const uint2 v = *reinterpret_cast<const uint2*>(p);
-          w[0] = v.x;
-          w[1] = v.y;
-        }
-        if constexpr (kWords == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(p);
-          w[0] = v.x;
-          w[1] = v.y;
-          w[2] = v.z;
-          w[3] = v.w;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (live && c + j < E) {
-          if constexpr (sizeof(T) == 4) w[j] = reinterpret_cast<const uint32_t*>(p)[j];
-          else w[j] = reinterpret_cast<const unsigned short*>(p)[j];
-        }
+    for (int j = 0; j < kVecs; ++j) {
+      v[j].clear();
+      if (live && c + j < E) v[j].load(p + j);
     }
   }
 };
@@ -784,41 +752,58 @@ __global__ void __launch_bounds__(256) k_ssm_bc(int64_t rows, int groups, const 
 }
 
 // --------------------------------------------------------------- one token
-template <typename T>
+// Four states of a channel a thread, for ROWS streams: A is read once for all of
+// them, and their states are in flight together.  VEC: B and C rows start on
+// four elements.
+template <typename T, int ROWS, bool VEC>
 __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
+  const int E = a.channels, per = E * 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t n = (int64_t)a.batch * a.channels * 4;
-  const bool on = i < n;
-  const int64_t be = (on ? i : n - 1) >> 2;
-  const int q = (int)(i & 3), E = a.channels;
-  const int64_t b = be / E;
-  const int e = (int)(be % E);
-  float4* st = reinterpret_cast<float4*>(a.state_out + be * kN + kQ * q);
-  const float4 h4 = *st;
-  const float4 A4 = *reinterpret_cast<const float4*>(a.A + (int64_t)e * kN + kQ * q);
-  const T* B = (const T*)a.B + b * a.B_bs + kQ * q;
-  const T* C = (const T*)a.C + b * a.C_bs + kQ * q;
-  const float x = to_f(((const T*)a.x)[b * a.x_bs + e]);
-  const float raw = to_f(((const T*)a.dt)[b * a.dt_bs + e]) + (a.dt_bias ? a.dt_bias[e] : 0.0f);
-  const float d = step_of(raw, a.softplus), du = d * x;
-  float h[4] = {h4.x, h4.y, h4.z, h4.w};
-  const float Av[4] = {A4.x, A4.y, A4.z, A4.w};
-  float v = 0.0f;
+  const int64_t b0 = i / per * ROWS;
+  const int r = (int)(i % per), e = r >> 2, q = r & 3;
+  // the four lanes of a channel take the same streams: per and the block are multiples of four
+  if (b0 >= a.batch) return;
+  const unsigned mask = 0xfu << (threadIdx.x & 28);
+  const int n = (int)min((int64_t)ROWS, a.batch - b0);
+  float4* const st = reinterpret_cast<float4*>(a.state_out + (b0 * E + e) * kN + kQ * q);
+  float4 h4[ROWS];
+  Row<T, 4, VEC> B[ROWS], C[ROWS];
+  T x[ROWS], dt[ROWS], z[ROWS];
 #pragma unroll
-  for (int j = 0; j < kQ; ++j) {
-    h[j] = fmaf(ex2(d * (Av[j] * kLog2e)), h[j], du * to_f(B[j]));
-    v = fmaf(to_f(C[j]), h[j], v);
-  }
-  if (on) *st = make_float4(h[0], h[1], h[2], h[3]);
-  v += __shfl_xor_sync(0xffffffffu, v, 2);
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  if (on && q == 0) {
-    if (a.D) v = fmaf(a.D[e], x, v);
-    if (a.z) {
-      const float z = to_f(((const T*)a.z)[b * a.z_bs + e]);
-      v *= z * sigmoid_f(z);
+  for (int k = 0; k < ROWS; ++k)
+    if (k < n) {
+      const int64_t b = b0 + k;
+      h4[k] = st[(int64_t)k * E * kQ];
+      B[k].load((const T*)a.B + b * a.B_bs + kQ * q, 0, 4, true);
+      C[k].load((const T*)a.C + b * a.C_bs + kQ * q, 0, 4, true);
+      x[k] = ((const T*)a.x)[b * a.x_bs + e];
+      dt[k] = ((const T*)a.dt)[b * a.dt_bs + e];
+      if (a.z) z[k] = ((const T*)a.z)[b * a.z_bs + e];
     }
-    ((T*)a.y)[be] = from_f<T>(v);
+  const float4 A4 = *reinterpret_cast<const float4*>(a.A + (int64_t)e * kN + kQ * q);
+  const float A2[4] = {A4.x * kLog2e, A4.y * kLog2e, A4.z * kLog2e, A4.w * kLog2e};
+  const float bias = a.dt_bias ? a.dt_bias[e] : 0.0f, D = a.D ? a.D[e] : 0.0f;
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    if (k >= n) break;
+    const float xk = to_f(x[k]), d = step_of(to_f(dt[k]) + bias, a.softplus), du = d * xk;
+    float h[4] = {h4[k].x, h4[k].y, h4[k].z, h4[k].w}, v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kQ; ++j) {
+      h[j] = fmaf(ex2(d * A2[j]), h[j], du * B[k].get(j));
+      v = fmaf(C[k].get(j), h[j], v);
+    }
+    st[(int64_t)k * E * kQ] = make_float4(h[0], h[1], h[2], h[3]);
+    v += __shfl_xor_sync(mask, v, 2);
+    v += __shfl_xor_sync(mask, v, 1);
+    if (q == 0) {
+      v = fmaf(D, xk, v);
+      if (a.z) {
+        const float zk = to_f(z[k]);
+        v *= zk * sigmoid_f(zk);
+      }
+      ((T*)a.y)[(b0 + k) * E + e] = from_f<T>(v);
+    }
   }
 }
 
@@ -933,6 +918,23 @@ static int ssm_backward(const boa_ssm_args& a, cudaStream_t s) {
   return ssm_vec(a, true) ? ssm_backward_t<T, true>(a, s) : ssm_backward_t<T, false>(a, s);
 }
 
+template <typename T, int ROWS>
+static void ssm_step_rows(const boa_ssm_args& a, cudaStream_t s) {
+  const int64_t n = (a.batch + ROWS - 1LL) / ROWS * a.channels * 4;
+  const unsigned grid = (unsigned)((n + 255) / 256);
+  if (row_vec(a.B, a.B_bs, 0, sizeof(T)) && row_vec(a.C, a.C_bs, 0, sizeof(T)))
+    k_ssm_step<T, ROWS, true><<<grid, 256, 0, s>>>(a);
+  else
+    k_ssm_step<T, ROWS, false><<<grid, 256, 0, s>>>(a);
+}
+
+// Four streams a thread where that still fills the GPU, else one.
+template <typename T>
+static void ssm_step_launch(const boa_ssm_args& a, cudaStream_t s) {
+  if ((int64_t)a.batch * a.channels * 4 >= 4 * 148LL * 2048) ssm_step_rows<T, 4>(a, s);
+  else ssm_step_rows<T, 1>(a, s);
+}
+
 static int ssm_check(const boa_ssm_args* a, const char* who) {
   if (!a) return boa_fail(BOA_ERR_ARG, std::string(who) + ": null arguments");
   if (a->batch < 0 || a->length < 0 || a->channels < 1)
@@ -1017,10 +1019,9 @@ BOA_API int boa_ssm_step(const boa_ssm_args* a, void* stream) {
     return boa_fail(BOA_ERR_ARG, "boa_ssm_step: state and A must be 16-byte aligned");
   BOA_CUDA(cudaSetDevice(a->device));
   cudaStream_t s = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)(((int64_t)a->batch * a->channels * 4 + 255) / 256);
-  if (a->dtype == BOA_DTYPE_F32) k_ssm_step<float><<<grid, 256, 0, s>>>(*a);
-  else if (a->dtype == BOA_DTYPE_BF16) k_ssm_step<__nv_bfloat16><<<grid, 256, 0, s>>>(*a);
-  else k_ssm_step<__half><<<grid, 256, 0, s>>>(*a);
+  if (a->dtype == BOA_DTYPE_F32) ssm_step_launch<float>(*a, s);
+  else if (a->dtype == BOA_DTYPE_BF16) ssm_step_launch<__nv_bfloat16>(*a, s);
+  else ssm_step_launch<__half>(*a, s);
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
 }
