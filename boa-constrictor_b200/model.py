@@ -12,6 +12,13 @@ dt in [1e-3, 1e-1] floored at 1e-4, A_log = log(1..16), D = 1.
 Inference (``init_stream`` / ``step`` / ``forward``) runs on the sm_100a kernel
 in libboa_b200.so (``boa_model_step`` / ``boa_model_logits``) on a CUDA
 device; there is no CPU execution path.
+
+``forward_layers`` / ``step_layers`` run the same model layer by layer on the
+module's own parameters (on the GPU, any d_model): the matrix products are
+torch's, everything between them is ``boa_b200.ops``.  This is the path with
+gradients, for prompts parallel over positions, and for ragged batches; its
+probabilities agree with the fused kernel's to rounding, not bit for bit, so the
+codec does not use it.
 """
 from __future__ import annotations
 
@@ -20,8 +27,10 @@ import math
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from boa_b200 import _native as _n
+from boa_b200 import ops
 from boa_b200.weights import flatten_state_dict
 
 D_STATE = 16
@@ -75,6 +84,42 @@ class Mamba(nn.Module):
         self.D = nn.Parameter(torch.ones(E))
         self.out_proj = nn.Linear(E, d_model, bias=False)
 
+    def init_state(self, batch_size: int, device=None, dtype=None):
+        """(convolution window [B, 3, E], scan state [B, E, 16] fp32) before the first token."""
+        w = self.in_proj.weight
+        device, dtype = device or w.device, dtype or w.dtype
+        return (torch.zeros(batch_size, D_CONV - 1, self.d_inner, dtype=dtype, device=device),
+                torch.zeros(batch_size, self.d_inner, D_STATE, dtype=torch.float32, device=device))
+
+    def _split(self, dbc):
+        return dbc.split([self.dt_rank, D_STATE, D_STATE], dim=-1)
+
+    def forward(self, u, state=None, lens=None, return_state: bool = False):
+        """u [B, L, d_model] -> [B, L, d_model], from ``state`` (zeros when None).
+        ``lens`` [B] cuts each row; with ``return_state`` also the state behind
+        every row's last valid position.  Differentiable."""
+        conv, ssm = (None, None) if state is None else state
+        x, z = self.in_proj(u).chunk(2, dim=-1)
+        x, conv = ops.causal_conv(x, self.conv1d.weight, self.conv1d.bias, state=conv, lens=lens, return_state=True)
+        dt, B, C = self._split(self.x_proj(x))
+        dt = F.linear(dt, self.dt_proj.weight)
+        y, ssm = ops.ssm_scan(x, dt, -torch.exp(self.A_log.float()), B, C, self.D, z, self.dt_proj.bias, state=ssm,
+                              lens=lens, return_state=True)
+        y = self.out_proj(y)
+        return (y, (conv, ssm)) if return_state else y
+
+    @torch.no_grad()
+    def step(self, u, state):
+        """One token of every stream: u [B, d_model] -> [B, d_model]; ``state``
+        (from ``init_state`` or ``forward``) moves on in place."""
+        conv, ssm = state
+        x, z = self.in_proj(u).chunk(2, dim=-1)
+        x = ops.causal_conv_step(x, conv, self.conv1d.weight, self.conv1d.bias)
+        dt, B, C = self._split(self.x_proj(x))
+        dt = F.linear(dt, self.dt_proj.weight)
+        y = ops.ssm_step(x, dt, ssm, -torch.exp(self.A_log.float()), B, C, self.D, z, self.dt_proj.bias)
+        return self.out_proj(y)
+
 
 class MambaBlock(nn.Module):
     """ln1 -> mamba -> ln2 -> ff -> + x (model.py:42-65)."""
@@ -85,6 +130,19 @@ class MambaBlock(nn.Module):
         self.mamba = Mamba(d_model)
         self.ln2 = nn.LayerNorm(d_model)
         self.ff = nn.Sequential(nn.Linear(d_model, 4 * d_model), nn.GELU(), nn.Linear(4 * d_model, d_model))
+
+    def _finish(self, x, y):
+        return x + self.ff(ops.layer_norm(y, self.ln2.weight, self.ln2.bias, self.ln2.eps))
+
+    def forward(self, x, state=None, lens=None, return_state: bool = False):
+        u = ops.layer_norm(x, self.ln1.weight, self.ln1.bias, self.ln1.eps)
+        y, state = self.mamba(u, state, lens, return_state=True)
+        y = self._finish(x, y)
+        return (y, state) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x, state):
+        return self._finish(x, self.mamba.step(ops.layer_norm(x, self.ln1.weight, self.ln1.bias, self.ln1.eps), state))
 
 
 class StreamState:
@@ -230,6 +288,44 @@ class BoaBytePredictor(nn.Module):
                     ctypes.c_void_p(out.data_ptr()), ctypes.c_void_p(ws.data_ptr()),
                     ctypes.c_size_t(ws.numel()), ctypes.c_void_p(_n.stream_ptr(dev)))
         return out
+
+
+    # -- layer by layer on the module's own parameters ---------------------------
+    def _check_tokens(self, who, x, dims):
+        if x.dim() != dims:
+            raise ValueError(f"{who}: tokens must be {'[batch, length]' if dims == 2 else '[batch]'}, "
+                             f"got {tuple(x.shape)}")
+        if not self.embedding.weight.is_cuda:
+            raise RuntimeError(f"{who} runs on CUDA devices only (no CPU path): move the model with .cuda()")
+
+    def forward_layers(self, x, state=None, lens=None, return_state: bool = False):
+        """x [B, L] -> logits [B, L, vocab], differentiable in every parameter.
+
+        ``lens`` [B] gives the valid length of each row (the logits behind it
+        are computed from zeros and mean nothing).  ``state`` continues a
+        sequence; with ``return_state`` the result is (logits, state behind
+        every row's last valid position) for a later call or ``step_layers``."""
+        self._check_tokens("forward_layers", x, 2)
+        h = self.embedding(x.to(self.embedding.weight.device).long())
+        out = []
+        for i, block in enumerate(self.blocks):
+            h, s = block(h, None if state is None else state[i], lens, return_state=True)
+            out.append(s)
+        logits = self.head(h)
+        return (logits, out) if return_state else logits
+
+    def init_layers(self, batch_size: int, dtype=None):
+        """The state before the first byte, for ``step_layers``."""
+        return [b.mamba.init_state(batch_size, dtype=dtype) for b in self.blocks]
+
+    @torch.no_grad()
+    def step_layers(self, byte_t, state):
+        """byte_t [B] -> logits [B, vocab]; ``state`` moves on in place."""
+        self._check_tokens("step_layers", byte_t, 1)
+        h = self.embedding(byte_t.to(self.embedding.weight.device).long())
+        for block, s in zip(self.blocks, state):
+            h = block.step(h, s)
+        return self.head(h)
 
 
 def BoaConstrictor(d_model=256, num_layers=4, vocab_size=256, device="cuda", weight_format: str | None = None):

@@ -3,8 +3,12 @@ loader of byte sequences, through the model's forward pass.
 
 BoaBytePredictor.forward runs the fused sm_100a kernel in logits mode with
 time blocks of 4 positions (the same kernel and weight tiles as compression),
-so evaluation costs one launch per batch instead of one per byte.  Training
-itself (train.py:24 onwards) is out of scope for this build and raises.
+so evaluation costs one launch per batch instead of one per byte.
+
+``train_step`` is one optimizer step on the layer-by-layer path
+(``BoaBytePredictor.forward_layers``), whose operators have backward kernels.
+The reference's training program around it (train.py:24 onwards: mixed
+precision, checkpoints every epoch) is out of scope for this build and raises.
 """
 from __future__ import annotations
 
@@ -28,6 +32,26 @@ def evaluate_bpp(model, loader, criterion, device="cuda", vocab_size=256) -> flo
         nll_sum += float(loss.item()) * targets.numel()
         count += targets.numel()
     return nll_sum / max(count, 1) / math.log(2.0)
+
+
+def train_step(model, batch, optimizer, criterion, lens=None) -> torch.Tensor:
+    """One step on a batch of byte rows [B, L]: predict bytes 1..L-1 from
+    0..L-2, ``criterion(logits, targets)``, backward, ``optimizer.step()``.
+    ``lens`` [B] is the number of valid bytes of each row; what lies behind
+    takes no part.  Returns the loss (on the device, nothing is synchronised)."""
+    dev = model.embedding.weight.device
+    batch = batch.to(dev)
+    inputs, targets = batch[:, :-1], batch[:, 1:].long()
+    if lens is not None:
+        lens = (lens.to(dev) - 1).clamp(min=0)
+        live = torch.arange(targets.shape[1], device=dev)[None, :] < lens[:, None]
+        targets = torch.where(live, targets, torch.full_like(targets, -100))     # cross_entropy's ignore_index
+    optimizer.zero_grad(set_to_none=True)
+    logits = model.forward_layers(inputs, lens=lens)
+    loss = criterion(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
+    loss.backward()
+    optimizer.step()
+    return loss.detach()
 
 
 def train(*args, **kwargs):
