@@ -452,6 +452,32 @@ def test_captured_and_replayed():
             assert torch.equal(o, want[i][k]), (i, j, k)
 
 
+def test_second_derivatives_are_refused():
+    ops = _ops()
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    y = ops.layer_norm(x, torch.ones(16, device="cuda"))
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_steps_refuse_gradients_and_saved_states_notice_them():
+    """The step forms change their state in place: they refuse gradients, and a graph that saved the state as it was
+    refuses to go back."""
+    ops = _ops()
+    c = _scan_case(2, 1, 16, F32, 60)
+    d = {k: _cuda(c[k]) for k in ("x", "dt", "A", "B", "C", "D", "z", "bias", "state")}
+    one = lambda k: d[k][:, 0]  # noqa: E731
+    step = lambda: ops.ssm_step(one("x"), one("dt"), d["state"], d["A"], one("B"), one("C"))  # noqa: E731
+    d["A"].requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        step()
+    y = ops.ssm_scan(d["x"], d["dt"], d["A"], d["B"], d["C"], state=d["state"])
+    with torch.no_grad():
+        step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_two_calls_on_two_streams():
     """The same call on two streams at once: no scratch is shared."""
     c = _scan_case(1, 2000, 64, F32, 50)
