@@ -810,20 +810,23 @@ __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
 // --------------------------------------------------------------------- host
 static int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
-// Parts of the length: one where the rows alone give enough blocks, else enough
-// for `want` blocks, no part shorter than 64 tokens.
-static SsmPlan ssm_plan(const boa_ssm_args& a, int64_t row_blocks, int64_t enough, int64_t want) {
+// Parts of the length for the forward call.  One where the rows alone give 256
+// blocks: at 256 blocks one part and many cost the same (203 and 202 us at 16 x
+// 2048 x 512; 54 and 67 us at 64 x 512 x 128), at 128 blocks many win (205
+// against 348 us at 8 x 4096 x 512), at 512 one does (554 against 692 us at 32 x
+// 4096 x 512).  Else enough parts for two rounds of the blocks that the SMs
+// hold, no part shorter than 64 tokens.
+static SsmPlan plan_forward(const boa_ssm_args& a) {
   SsmPlan p{};
   p.cblocks = (a.channels + kCh - 1) / kCh;
-  int parts = 1;
-  const int64_t blocks = (int64_t)a.batch * row_blocks;
-  if (blocks < enough) {
-    const int64_t most = (a.length + 63) / 64;
-    const int64_t need = (want + blocks - 1) / blocks;
-    parts = (int)(need < most ? need : most);
+  const int64_t blocks = (int64_t)a.batch * p.cblocks;
+  int64_t parts = 1;
+  if (blocks < 256) {
+    const int64_t most = (a.length + 63) / 64, need = (1776 + blocks - 1) / blocks;
+    parts = need < most ? need : most;
     if (parts < 1) parts = 1;
   }
-  p.part = round_up((a.length + parts - 1) / parts, kTile);
+  p.part = round_up((int)((a.length + parts - 1) / parts), kTile);
   if (p.part < kTile) p.part = kTile;
   p.parts = a.length > 0 ? (a.length + p.part - 1) / p.part : 1;
   return p;
@@ -837,8 +840,29 @@ static int back_groups(const boa_ssm_args& a) {
   const int per = back_passes(a) * kBackCh;
   return (a.channels + per - 1) / per;
 }
-static SsmPlan plan_forward(const boa_ssm_args& a) { return ssm_plan(a, (a.channels + kCh - 1) / kCh, 888, 1776); }
-static SsmPlan plan_backward(const boa_ssm_args& a) { return ssm_plan(a, back_groups(a), 444, 592); }
+// Parts for the backward call, whose blocks have an SM each: of 1 to 8 rounds of
+// 148 blocks, the one with the least tokens to walk one after the other (about
+// 6 tokens' time a block for its start and end), more rounds where they cost
+// at most 3 % more, since rows of different lengths then even out.
+static SsmPlan plan_backward(const boa_ssm_args& a) {
+  SsmPlan p{};
+  p.cblocks = (a.channels + kCh - 1) / kCh;
+  const int64_t blocks = (int64_t)a.batch * back_groups(a), most = (a.length + 31) / 32;
+  int64_t best = -1;
+  for (int rounds = 1; rounds <= 8; ++rounds) {
+    int64_t parts = 148LL * rounds / blocks;
+    parts = parts < 1 ? 1 : parts < most ? parts : most < 1 ? 1 : most;
+    const int part = round_up((int)((a.length + parts - 1) / parts), kBack);
+    const int n = part > 0 ? (a.length + part - 1) / part : 1;
+    const int64_t cost = (blocks * n + 147) / 148 * (part + 6);
+    if (best < 0 || cost * 100 <= best * 103) {
+      p.part = part > kBack ? part : kBack;
+      p.parts = n > 1 ? n : 1;
+      best = best < 0 || cost < best ? cost : best;
+    }
+  }
+  return p;
+}
 
 // Vector accesses where every row of every tensor starts on four elements.
 static bool row_vec(const void* p, int64_t bs, int64_t ts, size_t size) {
