@@ -216,6 +216,19 @@ __device__ __forceinline__ f2 ex2_2(f2 a) {
   return pack(ex2(t.x), ex2(t.y));
 }
 
+// softplus_f of two values; u as there.
+__device__ __forceinline__ f2 softplus2(f2 v, f2& u) {
+  u = ex2_2(mul2(f2{v.v & 0x7fffffff7fffffffull}, pack(-kLog2e, -kLog2e)));
+  const float2 den = unpack(add2(u, pack(2.0f, 2.0f)));
+  const f2 s = mul2(u, pack(rcp(den.x), rcp(den.y))), w = mul2(s, s);
+  f2 p = fma2(pack(0.14089173f, 0.14089173f), w, pack(0.13980299f, 0.13980299f));
+  p = fma2(p, w, pack(0.20012455f, 0.20012455f));
+  p = fma2(p, w, pack(0.33333158f, 0.33333158f));
+  p = fma2(p, w, pack(1.0f, 1.0f));
+  const float2 x = unpack(v);
+  return fma2(add2(s, s), p, pack(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+}
+
 // V fp32 values of neighbouring channels: pairs where V is even, one value for V = 1.
 template <int V>
 struct Fv {

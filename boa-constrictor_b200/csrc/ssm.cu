@@ -62,11 +62,32 @@ __device__ __forceinline__ void store_row(T* p, int c, int E, const float (&v)[V
       if (c + j < E) p[j] = from_f<T>(v[j]);
   }
 }
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_row2(T* p, int c, int E, const f2 (&v)[2]) {
+  const float2 a = unpack(v[0]), b = unpack(v[1]);
+  const float x[4] = {a.x, a.y, b.x, b.y};
+  store_row<T, 4, VEC>(p, c, E, x);
+}
+// Four values of shared memory as two pairs.
+__device__ __forceinline__ void ld2(const float* p, f2 (&v)[2]) {
+  const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(p);
+  v[0] = f2{r.x};
+  v[1] = f2{r.y};
+}
+__device__ __forceinline__ void st2(float* p, const f2 (&v)[2]) {
+  *reinterpret_cast<ulonglong2*>(p) = make_ulonglong2(v[0].v, v[1].v);
+}
 // Parameters of V channels, zeros beyond the last or without the array.
 template <int V>
 __device__ __forceinline__ void load_params(const float* p, int c, int E, float (&v)[V]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = p && c + j < E ? p[c + j] : 0.0f;
+}
+__device__ __forceinline__ void load_pairs(const float* p, int c, int E, f2 (&v)[2]) {
+  float t[4];
+  load_params<4>(p, c, E, t);
+  v[0] = pack(t[0], t[1]);
+  v[1] = pack(t[2], t[3]);
 }
 __device__ __forceinline__ float step_of(float raw, bool softplus) {
   float u;
@@ -99,8 +120,9 @@ struct SsmPlan {
 template <typename T, bool ENDS, bool VEC>
 __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const SsmPlan p, float* __restrict__ ends,
                                                      float* __restrict__ dsum) {
-  __shared__ __align__(16) float sd[kTile][kPitch], su[kTile][kPitch], sy[kTile][kPitch];
-  __shared__ __align__(16) float sbc[kTile][2 * kN];
+  // d and d x of every token and channel, twice each, as the paired operations take them
+  __shared__ __align__(16) f2 sd[kTile][kCh], su[kTile][kCh];
+  __shared__ __align__(16) float sy[kTile][kPitch], sbc[kTile][2 * kN];
   const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
   const int nparts = ENDS ? p.parts - 1 : p.parts;
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
@@ -121,9 +143,9 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
                       : (const T*)a.B + b * a.B_bs + t * a.B_ts + 4 * sub;
   const int64_t bcts = is_c ? a.C_ts : a.B_ts;
   T* py = (T*)a.y + ((int64_t)b * a.length + t) * E + c;
-  float bias[4], Dv[4];
-  load_params<4>(a.dt_bias, c, E, bias);
-  load_params<4>(a.D, c, E, Dv);
+  f2 bias[2], Dv[2];
+  load_pairs(a.dt_bias, c, E, bias);
+  load_pairs(a.D, c, E, Dv);
   f2 A2[2], h[2];
   {
     float v[kQ], s[kQ];
@@ -141,7 +163,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
   const int nck = (a.length + kBack - 1) / kBack;
   float* ck = !ENDS && a.checkpoints && on
                   ? a.checkpoints + (((int64_t)b * nck + begin / kBack) * E + e) * kN + kQ * q : nullptr;
-  float total = 0.0f;
+  f2 total{0ull};
   Row<T, 4, VEC> rx, rd, rz, rb;
   auto fetch = [&]() {
     const bool live = t < end;
@@ -156,15 +178,18 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
   };
   if (begin < end) fetch();
   for (int t0 = begin; t0 < end; t0 += kTile) {
-    float xs[4], zs[4], d[4];
+    f2 xs[2], zs[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      xs[j] = rx.get(j);
-      zs[j] = gated ? rz.get(j) : 0.0f;
-      d[j] = t < end ? step_of(rd.get(j) + bias[j], a.softplus) : 0.0f;
+    for (int j = 0; j < 2; ++j) {
+      xs[j] = pack(rx.get(2 * j), rx.get(2 * j + 1));
+      zs[j] = gated ? pack(rz.get(2 * j), rz.get(2 * j + 1)) : f2{0ull};
+      f2 d = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]), u;
+      if (a.softplus) d = softplus2(d, u);
+      if (t >= end) d = f2{0ull};
+      const float2 dv = unpack(d), uv = unpack(mul2(d, xs[j]));
+      *reinterpret_cast<float4*>(&sd[row][4 * sub + 2 * j]) = make_float4(dv.x, dv.x, dv.y, dv.y);
+      *reinterpret_cast<float4*>(&su[row][4 * sub + 2 * j]) = make_float4(uv.x, uv.x, uv.y, uv.y);
     }
-    *reinterpret_cast<float4*>(&sd[row][4 * sub]) = make_float4(d[0], d[1], d[2], d[3]);
-    *reinterpret_cast<float4*>(&su[row][4 * sub]) = make_float4(d[0] * xs[0], d[1] * xs[1], d[2] * xs[2], d[3] * xs[3]);
     *reinterpret_cast<float4*>(&sbc[row][4 * sub]) = make_float4(rb.get(0), rb.get(1), rb.get(2), rb.get(3));
     const bool mine = t < stop, live = t < end;
     t += kTile;
@@ -179,13 +204,12 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float dk = sd[u + k][ch], uk = su[u + k][ch];
-        const f2 dd = pack(dk, dk), uu = pack(uk, uk);
+        const f2 dd = sd[u + k][ch], uu = su[u + k][ch];
         const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sbc[u + k][kQ * q]);
         h[0] = fma2(ex2_2(mul2(dd, A2[0])), h[0], mul2(uu, f2{B.x}));
         h[1] = fma2(ex2_2(mul2(dd, A2[1])), h[1], mul2(uu, f2{B.y}));
         if constexpr (ENDS) {
-          total += dk;
+          total = add2(total, dd);
         } else {
           const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sbc[u + k][kN + kQ * q]);
           const float2 y = unpack(fma2(f2{C.x}, h[0], mul2(f2{C.y}, h[1])));
@@ -198,13 +222,14 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
     if constexpr (!ENDS) {
       if (mine) {
         float o[4];
-        const float4 v = *reinterpret_cast<const float4*>(&sy[row][4 * sub]);
-        const float vv[4] = {v.x, v.y, v.z, v.w};
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sy[row][4 * sub]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          o[j] = fmaf(Dv[j], xs[j], vv[j]);
-          if (gated) o[j] *= zs[j] * sigmoid_f(zs[j]);
-          if (!live) o[j] = 0.0f;
+        for (int j = 0; j < 2; ++j) {
+          f2 y = fma2(Dv[j], xs[j], f2{j ? v.y : v.x});
+          if (gated) y = mul2(y, mul2(zs[j], vsigmoid<2>(Fv<2>{{zs[j]}}).p[0]));
+          const float2 r = unpack(y);
+          o[2 * j] = live ? r.x : 0.0f;
+          o[2 * j + 1] = live ? r.y : 0.0f;
         }
         store_row<T, 4, VEC>(py, c, E, o);
       }
@@ -214,7 +239,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
   if constexpr (ENDS) {
     if (on) {
       *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(h[0].v, h[1].v);
-      if (q == 0) dsum[slot] = total;
+      if (q == 0) dsum[slot] = unpack(total).x;
     }
   } else {
     const float zero[4] = {};
@@ -272,7 +297,7 @@ static __global__ void __launch_bounds__(128) k_ssm_join(int64_t n, int E, int p
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_args a, const SsmPlan p,
                                                                float* __restrict__ ends, float* __restrict__ dsum) {
-  __shared__ __align__(16) float sd[kTile][kPitch], sg[kTile][kPitch];
+  __shared__ __align__(16) f2 sd[kTile][kCh], sg[kTile][kCh];
   __shared__ __align__(16) float sc[kTile][kN];
   const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
@@ -288,8 +313,8 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
   const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
   const T* pz = (const T*)a.z + b * a.z_bs + t * a.z_ts + c;
   const T* pc = (const T*)a.C + b * a.C_bs + t * a.C_ts + 4 * sub;   // lanes with sub < 4
-  float bias[4];
-  load_params<4>(a.dt_bias, c, E, bias);
+  f2 bias[2];
+  load_pairs(a.dt_bias, c, E, bias);
   f2 A2[2], g2[2] = {pack(0.f, 0.f), pack(0.f, 0.f)};
   {
     float v[kQ];
@@ -298,7 +323,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
     A2[0] = pack(v[0], v[1]);
     A2[1] = pack(v[2], v[3]);
   }
-  float total = 0.0f;
+  f2 total{0ull};
   Row<T, 4, VEC> rg, rd, rz, rc;
   auto fetch = [&]() {
     const bool live = t < end;
@@ -313,18 +338,19 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
   };
   if (tiles) fetch();
   for (int k = tiles - 1; k >= 0; --k) {
-    float d[4], g[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      g[j] = rg.get(j);
+    for (int j = 0; j < 2; ++j) {
+      f2 d = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]), u, g = pack(rg.get(2 * j), rg.get(2 * j + 1));
+      if (a.softplus) d = softplus2(d, u);
+      if (t >= end) d = f2{0ull};
       if (gated) {
-        const float z = rz.get(j);
-        g[j] *= z * sigmoid_f(z);
+        const f2 z = pack(rz.get(2 * j), rz.get(2 * j + 1));
+        g = mul2(g, mul2(z, vsigmoid<2>(Fv<2>{{z}}).p[0]));
       }
-      d[j] = t < end ? step_of(rd.get(j) + bias[j], a.softplus) : 0.0f;
+      const float2 dv = unpack(d), gv = unpack(g);
+      *reinterpret_cast<float4*>(&sd[row][4 * sub + 2 * j]) = make_float4(dv.x, dv.x, dv.y, dv.y);
+      *reinterpret_cast<float4*>(&sg[row][4 * sub + 2 * j]) = make_float4(gv.x, gv.x, gv.y, gv.y);
     }
-    *reinterpret_cast<float4*>(&sd[row][4 * sub]) = make_float4(d[0], d[1], d[2], d[3]);
-    *reinterpret_cast<float4*>(&sg[row][4 * sub]) = make_float4(g[0], g[1], g[2], g[3]);
     if (sub < 4)
       *reinterpret_cast<float4*>(&sc[row][4 * sub]) = make_float4(rc.get(0), rc.get(1), rc.get(2), rc.get(3));
     t -= kTile;
@@ -332,18 +358,17 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
     if (k > 0) fetch();
 #pragma unroll
     for (int i = kTile - 1; i >= 0; --i) {
-      const float dk = sd[i][ch], gk = sg[i][ch];
-      const f2 dd = pack(dk, dk), gg = pack(gk, gk);
+      const f2 dd = sd[i][ch], gg = sg[i][ch];
       const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sc[i][kQ * q]);
       g2[0] = mul2(ex2_2(mul2(dd, A2[0])), fma2(f2{C.x}, gg, g2[0]));
       g2[1] = mul2(ex2_2(mul2(dd, A2[1])), fma2(f2{C.y}, gg, g2[1]));
-      total += dk;
+      total = add2(total, dd);
     }
     __syncthreads();
   }
   if (on) {
     *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(g2[0].v, g2[1].v);
-    if (q == 0) dsum[slot] = total;
+    if (q == 0) dsum[slot] = unpack(total).x;
   }
 }
 
@@ -620,32 +645,35 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         pck -= ((int64_t)E + back) * kN;
       }
     };
-    float ps[4], pz4[4], pxv[4], pdv[4], pgv[4];     // of the pass staged before: sigmoid, dy silu'(z), x, d, g
+    f2 ps[2], pz2[2], px2[2], pd2[2], pg2[2];   // of the pass staged before: sigmoid, dy silu'(z), x, d, g
+    const f2 one = pack(1.0f, 1.0f), minus = pack(-1.0f, -1.0f), ln2 = pack(kLn2, kLn2);
     auto finish = [&](int slot, int g, bool store, bool in_row) {
       bar_sync(kDone + slot, kBackThreads);
       const float* const sums = sm + slot * S::kSlot + S::sums + row * kBackPitch + cl;
-      const int at = row * width + g * kBackCh + cl;
-      const float4 s1 = ld4(sums), s2 = ld4(sums + S::kSums), sv = ld4(sums + 2 * S::kSums);
-      const float4 D4 = ld4(D_s + g * kBackCh + cl), aD = ld4(dD_s + at), ab = ld4(db_s + at);
-      const float s1v[4] = {s1.x, s1.y, s1.z, s1.w}, s2v[4] = {s2.x, s2.y, s2.z, s2.w};
-      const float svv[4] = {sv.x, sv.y, sv.z, sv.w}, Dv[4] = {D4.x, D4.y, D4.z, D4.w};
-      float accD[4] = {aD.x, aD.y, aD.z, aD.w}, accb[4] = {ab.x, ab.y, ab.z, ab.w};
-      float ox[4], od[4], oz[4];
+      float* const dD = dD_s + row * width + g * kBackCh + cl;
+      float* const db = db_s + row * width + g * kBackCh + cl;
+      f2 s1[2], s2[2], sv[2], Dv[2], aD[2], ab[2], ox[2], od[2], oz[2];
+      ld2(sums, s1);
+      ld2(sums + S::kSums, s2);
+      ld2(sums + 2 * S::kSums, sv);
+      ld2(D_s + g * kBackCh + cl, Dv);
+      ld2(dD, aD);
+      ld2(db, ab);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ox[j] = fmaf(s1v[j], pdv[j], Dv[j] * pgv[j]);
-        od[j] = in_row ? fmaf(s1v[j], pxv[j], kLn2 * s2v[j]) * ps[j] : 0.0f;   // s2 is in units of log2
-        oz[j] = gated ? pz4[j] * fmaf(Dv[j], pxv[j], svv[j]) : 0.0f;
-        accD[j] = fmaf(pgv[j], pxv[j], accD[j]);
-        accb[j] += od[j];
+      for (int j = 0; j < 2; ++j) {
+        ox[j] = fma2(s1[j], pd2[j], mul2(Dv[j], pg2[j]));
+        od[j] = in_row ? mul2(fma2(s1[j], px2[j], mul2(ln2, s2[j])), ps[j]) : f2{0ull};   // s2 is in units of log2
+        oz[j] = gated ? mul2(pz2[j], fma2(Dv[j], px2[j], sv[j])) : f2{0ull};
+        aD[j] = fma2(pg2[j], px2[j], aD[j]);
+        ab[j] = add2(ab[j], od[j]);
       }
-      st4(dD_s + at, make_float4(accD[0], accD[1], accD[2], accD[3]));
-      st4(db_s + at, make_float4(accb[0], accb[1], accb[2], accb[3]));
+      st2(dD, aD);
+      st2(db, ab);
       if (store) {
         const int oc = e0 + g * kBackCh + cl;
-        store_row<T, 4, VEC>((T*)a.dx + out, oc, E, ox);
-        store_row<T, 4, VEC>((T*)a.ddt + out, oc, E, od);
-        if (gated) store_row<T, 4, VEC>((T*)a.dz + out, oc, E, oz);
+        store_row2<T, VEC>((T*)a.dx + out, oc, E, ox);
+        store_row2<T, VEC>((T*)a.ddt + out, oc, E, od);
+        if (gated) store_row2<T, VEC>((T*)a.dz + out, oc, E, oz);
       }
       out += kBackCh;
       if (g == np - 1) out -= (int64_t)kBack * E + np * kBackCh;
@@ -657,37 +685,39 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       const int ts = begin + k * kBack + row;
       const bool in_row = ts < end;
       for (int g = 0; g < np; ++g) {
-        const float4 b4 = ld4(bias_s + g * kBackCh + cl);
-        const float bias[4] = {b4.x, b4.y, b4.z, b4.w};
-        float sg[4], dz[4], xs[4], ds[4], gs[4];
+        f2 bias[2], sg[2], dz[2], xs[2], ds[2], gs[2];
+        ld2(bias_s + g * kBackCh + cl, bias);
         float* const sl = sm + slot * S::kSlot;
         float* const in = sl + 4 * (row * kBackCh + cl);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float raw = rd.get(j) + bias[j], x = rx.get(j);
-          float d = raw, g1 = rg.get(j);
-          sg[j] = 1.0f;
-          dz[j] = 0.0f;
-          if (a.softplus) {
-            float u;
-            d = softplus_f(raw, u);
-            sg[j] = (raw >= 0.0f ? 1.0f : u) * rcp(1.0f + u);
-          }
-          if (!in_row || e0 + g * kBackCh + cl + j >= E) d = 0.0f;
-          if (gated) {
-            const float z = rz.get(j), s = sigmoid_f(z);
-            dz[j] = g1 * (s * (1.0f + z * (1.0f - s)));
-            g1 *= z * s;
-          }
-          const float u = d * x;
-          st4(in + 4 * j, make_float4(d, d, u, u));
-          ds[j] = d;
-          gs[j] = g1;
-          xs[j] = x;
-        }
         float* const gg = sl + S::gg + 2 * (row * kBackCh + cl);
-        st4(gg, make_float4(gs[0], gs[0], gs[1], gs[1]));
-        st4(gg + 4, make_float4(gs[2], gs[2], gs[3], gs[3]));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f2 raw = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]);
+          xs[j] = pack(rx.get(2 * j), rx.get(2 * j + 1));
+          gs[j] = pack(rg.get(2 * j), rg.get(2 * j + 1));
+          f2 d = raw;
+          sg[j] = one;
+          dz[j] = f2{0ull};
+          if (a.softplus) {
+            f2 u;
+            d = softplus2(raw, u);
+            // sigmoid(raw) = (raw >= 0 ? 1 : u) / (1 + u), u = exp(-|raw|)
+            const float2 r = unpack(raw), uv = unpack(u), q = unpack(add2(u, one));
+            sg[j] = pack((r.x >= 0.0f ? 1.0f : uv.x) * rcp(q.x), (r.y >= 0.0f ? 1.0f : uv.y) * rcp(q.y));
+          }
+          if (!in_row) d = f2{0ull};
+          if (gated) {
+            const f2 z = pack(rz.get(2 * j), rz.get(2 * j + 1)), s = vsigmoid<2>(Fv<2>{{z}}).p[0], zs = mul2(z, s);
+            // silu'(z) = s + z s (1 - s)
+            dz[j] = mul2(gs[j], fma2(zs, fma2(s, minus, one), s));
+            gs[j] = mul2(gs[j], zs);
+          }
+          const float2 dv = unpack(d), uv = unpack(mul2(d, xs[j])), gv = unpack(gs[j]);
+          st4(in + 8 * j, make_float4(dv.x, dv.x, uv.x, uv.x));
+          st4(in + 8 * j + 4, make_float4(dv.y, dv.y, uv.y, uv.y));
+          st4(gg + 4 * j, make_float4(gv.x, gv.x, gv.y, gv.y));
+          ds[j] = d;
+        }
         st4(sl + S::h0 + 4 * tid, rh[0]);
         st4(sl + S::h0 + 32 * kN + 4 * tid, rh[1]);
         if (g == 0)
@@ -702,12 +732,12 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         }
         have = true;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           ps[j] = sg[j];
-          pz4[j] = dz[j];
-          pxv[j] = xs[j];
-          pdv[j] = ds[j];
-          pgv[j] = gs[j];
+          pz2[j] = dz[j];
+          px2[j] = xs[j];
+          pd2[j] = ds[j];
+          pg2[j] = gs[j];
         }
         slot ^= 1;
       }
