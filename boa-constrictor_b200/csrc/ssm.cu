@@ -68,6 +68,8 @@ __device__ __forceinline__ void store_row2(T* p, int c, int E, const f2 (&v)[2])
   const float x[4] = {a.x, a.y, b.x, b.y};
   store_row<T, 4, VEC>(p, c, E, x);
 }
+__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ void st4(void* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 // Four values of shared memory as two pairs.
 __device__ __forceinline__ void ld2(const float* p, f2 (&v)[2]) {
   const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(p);
@@ -116,136 +118,75 @@ struct SsmPlan {
 };
 
 // ------------------------------------------------------------------ forward
-// ENDS: only the part's end state (from zero) and sum of d, into ends / dsum.
-template <typename T, bool ENDS, bool VEC>
-__global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const SsmPlan p, float* __restrict__ ends,
-                                                     float* __restrict__ dsum) {
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+enum { kFull = 1, kDone = 3, kScanOnly = 5 };          // barrier ids; kFull and kDone one per slot
+
+constexpr int kScanThreads = 2 * kSsmThreads;
+
+// One pass over a part: warps 4-7 stage a tile (softplus once an element) and
+// finish it (D x and the gate), warps 0-3 carry h through it.  The two work on
+// neighbouring tiles, two slots of shared memory apart.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kScanThreads, 4) k_ssm(const boa_ssm_args a, const SsmPlan p,
+                                                         const float* __restrict__ starts) {
   // d and d x of every token and channel, twice each, as the paired operations take them
-  __shared__ __align__(16) f2 sd[kTile][kCh], su[kTile][kCh];
-  __shared__ __align__(16) float sy[kTile][kPitch], sbc[kTile][2 * kN];
-  const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
-  const int nparts = ENDS ? p.parts - 1 : p.parts;
+  __shared__ __align__(16) f2 sd[2][kTile][kCh], su[2][kTile][kCh];
+  __shared__ __align__(16) float sy[2][kTile][kPitch], sbc[2][kTile][2 * kN];
+  const int tid = threadIdx.x & (kSsmThreads - 1);
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
-  const int part = (blockIdx.x / p.cblocks) % nparts, b = blockIdx.x / p.cblocks / nparts;
-  const int e = e0 + ch;
-  const bool on = e < E, gated = !ENDS && a.z;
+  const int part = (blockIdx.x / p.cblocks) % p.parts, b = blockIdx.x / p.cblocks / p.parts;
   const int len = row_len(a, b);
   const int begin = part * p.part, stop = min(begin + p.part, a.length), end = min(stop, len);
-  const int64_t slot = ((int64_t)b * p.parts + part) * E + e;
-  // staging: a thread moves four channels of token `row`, and four values of its B or C
-  const int row = tid >> 3, sub = tid & 7, c = e0 + 4 * sub;
-  const bool is_c = sub >= 4;
-  int t = begin + row;
-  const T* px = (const T*)a.x + b * a.x_bs + t * a.x_ts + c;
-  const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
-  const T* pz = (const T*)a.z + b * a.z_bs + t * a.z_ts + c;
-  const T* pbc = is_c ? (const T*)a.C + b * a.C_bs + t * a.C_ts + 4 * (sub - 4)
-                      : (const T*)a.B + b * a.B_bs + t * a.B_ts + 4 * sub;
-  const int64_t bcts = is_c ? a.C_ts : a.B_ts;
-  T* py = (T*)a.y + ((int64_t)b * a.length + t) * E + c;
-  f2 bias[2], Dv[2];
-  load_pairs(a.dt_bias, c, E, bias);
-  load_pairs(a.D, c, E, Dv);
-  f2 A2[2], h[2];
-  {
-    float v[kQ], s[kQ];
-    const float* s0 = ENDS ? nullptr : p.parts > 1 ? ends + slot * kN : a.state ? a.state + ((int64_t)b * E + e) * kN : nullptr;
+  int slot = 0;
+  if (threadIdx.x < kSsmThreads) {
+    const int lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane), e = e0 + ch;
+    const bool on = e < E;
+    f2 A2[2], h[2];
+    {
+      float v[kQ], s[kQ];
+      const float* s0 = p.parts > 1 ? starts + (((int64_t)b * p.parts + part) * E + e) * kN
+                        : a.state   ? a.state + ((int64_t)b * E + e) * kN : nullptr;
 #pragma unroll
-    for (int j = 0; j < kQ; ++j) {
-      v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
-      s[j] = on && s0 ? s0[kQ * q + j] : 0.0f;
-    }
-    A2[0] = pack(v[0], v[1]);
-    A2[1] = pack(v[2], v[3]);
-    h[0] = pack(s[0], s[1]);
-    h[1] = pack(s[2], s[3]);
-  }
-  const int nck = (a.length + kBack - 1) / kBack;
-  float* ck = !ENDS && a.checkpoints && on
-                  ? a.checkpoints + (((int64_t)b * nck + begin / kBack) * E + e) * kN + kQ * q : nullptr;
-  f2 total{0ull};
-  Row<T, 4, VEC> rx, rd, rz, rb;
-  auto fetch = [&]() {
-    const bool live = t < end;
-    rx.load(px, c, E, live);
-    rd.load(pd, c, E, live);
-    if (gated) rz.load(pz, c, E, live);
-    rb.load(pbc, 0, 4, live && !(ENDS && is_c));
-    px += kTile * a.x_ts;
-    pd += kTile * a.dt_ts;
-    pz += kTile * a.z_ts;
-    pbc += kTile * bcts;
-  };
-  if (begin < end) fetch();
-  for (int t0 = begin; t0 < end; t0 += kTile) {
-    f2 xs[2], zs[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      xs[j] = pack(rx.get(2 * j), rx.get(2 * j + 1));
-      zs[j] = gated ? pack(rz.get(2 * j), rz.get(2 * j + 1)) : f2{0ull};
-      f2 d = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]), u;
-      if (a.softplus) d = softplus2(d, u);
-      if (t >= end) d = f2{0ull};
-      const float2 dv = unpack(d), uv = unpack(mul2(d, xs[j]));
-      *reinterpret_cast<float4*>(&sd[row][4 * sub + 2 * j]) = make_float4(dv.x, dv.x, dv.y, dv.y);
-      *reinterpret_cast<float4*>(&su[row][4 * sub + 2 * j]) = make_float4(uv.x, uv.x, uv.y, uv.y);
-    }
-    *reinterpret_cast<float4*>(&sbc[row][4 * sub]) = make_float4(rb.get(0), rb.get(1), rb.get(2), rb.get(3));
-    const bool mine = t < stop, live = t < end;
-    t += kTile;
-    __syncthreads();
-    if (t0 + kTile < end) fetch();
-#pragma unroll
-    for (int u = 0; u < kTile; u += 4) {
-      float yp[4];
-      if (!ENDS && u % kBack == 0 && ck && t0 + u < end) {
-        *reinterpret_cast<ulonglong2*>(ck) = make_ulonglong2(h[0].v, h[1].v);
-        ck += (int64_t)E * kN;
+      for (int j = 0; j < kQ; ++j) {
+        v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+        s[j] = on && s0 ? s0[kQ * q + j] : 0.0f;
       }
+      A2[0] = pack(v[0], v[1]);
+      A2[1] = pack(v[2], v[3]);
+      h[0] = pack(s[0], s[1]);
+      h[1] = pack(s[2], s[3]);
+    }
+    const int nck = (a.length + kBack - 1) / kBack;
+    float* ck = a.checkpoints && on
+                    ? a.checkpoints + (((int64_t)b * nck + begin / kBack) * E + e) * kN + kQ * q : nullptr;
+    for (int t0 = begin; t0 < end; t0 += kTile) {
+      bar_sync(kFull + slot, kScanThreads);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f2 dd = sd[u + k][ch], uu = su[u + k][ch];
-        const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sbc[u + k][kQ * q]);
-        h[0] = fma2(ex2_2(mul2(dd, A2[0])), h[0], mul2(uu, f2{B.x}));
-        h[1] = fma2(ex2_2(mul2(dd, A2[1])), h[1], mul2(uu, f2{B.y}));
-        if constexpr (ENDS) {
-          total = add2(total, dd);
-        } else {
-          const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sbc[u + k][kN + kQ * q]);
+      for (int u = 0; u < kTile; u += 4) {
+        float yp[4];
+        if (u % kBack == 0 && ck && t0 + u < end) {
+          *reinterpret_cast<ulonglong2*>(ck) = make_ulonglong2(h[0].v, h[1].v);
+          ck += (int64_t)E * kN;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f2 dd = sd[slot][u + k][ch], uu = su[slot][u + k][ch];
+          const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sbc[slot][u + k][kQ * q]);
+          const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sbc[slot][u + k][kN + kQ * q]);
+          h[0] = fma2(ex2_2(mul2(dd, A2[0])), h[0], mul2(uu, f2{B.x}));
+          h[1] = fma2(ex2_2(mul2(dd, A2[1])), h[1], mul2(uu, f2{B.y}));
           const float2 y = unpack(fma2(f2{C.x}, h[0], mul2(f2{C.y}, h[1])));
           yp[k] = y.x + y.y;
         }
+        sy[slot][u + q][ch] = quad_sum(yp, q);
       }
-      if constexpr (!ENDS) sy[u + q][ch] = quad_sum(yp, q);
-    }
-    __syncthreads();
-    if constexpr (!ENDS) {
-      if (mine) {
-        float o[4];
-        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sy[row][4 * sub]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          f2 y = fma2(Dv[j], xs[j], f2{j ? v.y : v.x});
-          if (gated) y = mul2(y, mul2(zs[j], vsigmoid<2>(Fv<2>{{zs[j]}}).p[0]));
-          const float2 r = unpack(y);
-          o[2 * j] = live ? r.x : 0.0f;
-          o[2 * j + 1] = live ? r.y : 0.0f;
-        }
-        store_row<T, 4, VEC>(py, c, E, o);
-      }
-      py += (int64_t)kTile * E;
-    }
-  }
-  if constexpr (ENDS) {
-    if (on) {
-      *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(h[0].v, h[1].v);
-      if (q == 0) dsum[slot] = unpack(total).x;
-    }
-  } else {
-    const float zero[4] = {};
-    for (; t < stop; t += kTile) {   // tiles wholly behind the row's end
-      store_row<T, 4, VEC>(py, c, E, zero);
-      py += (int64_t)kTile * E;
+      bar_arrive(kDone + slot, kScanThreads);
+      slot ^= 1;
     }
     if (a.state_out && part == p.parts - 1 && on) {
       float* so = a.state_out + ((int64_t)b * E + e) * kN + kQ * q;
@@ -255,6 +196,156 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm(const boa_ssm_args a, const
       so[2] = hi.x;
       so[3] = hi.y;
     }
+  } else {
+    // a thread moves four channels of token `row` of a tile, and four values of its B or C
+    const bool gated = a.z;
+    const int row = tid >> 3, sub = tid & 7, c = e0 + 4 * sub;
+    const bool is_c = sub >= 4;
+    int t = begin + row;                       // of the tile to be loaded next
+    const T* px = (const T*)a.x + b * a.x_bs + t * a.x_ts + c;
+    const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
+    const T* pz = (const T*)a.z + b * a.z_bs + t * a.z_ts + c;
+    const T* pbc = is_c ? (const T*)a.C + b * a.C_bs + t * a.C_ts + 4 * (sub - 4)
+                        : (const T*)a.B + b * a.B_bs + t * a.B_ts + 4 * sub;
+    const int64_t bcts = is_c ? a.C_ts : a.B_ts;
+    T* py = (T*)a.y + ((int64_t)b * a.length + t) * E + c;
+    f2 bias[2], Dv[2], px2[2], pz2[2];         // x and z of the tile staged before
+    load_pairs(a.dt_bias, c, E, bias);
+    load_pairs(a.D, c, E, Dv);
+    Row<T, 4, VEC> rx, rd, rz, rb;
+    auto fetch = [&]() {
+      const bool live = t < end;
+      rx.load(px, c, E, live);
+      rd.load(pd, c, E, live);
+      if (gated) rz.load(pz, c, E, live);
+      rb.load(pbc, 0, 4, live);
+      px += kTile * a.x_ts;
+      pd += kTile * a.dt_ts;
+      pz += kTile * a.z_ts;
+      pbc += kTile * bcts;
+      t += kTile;
+    };
+    auto finish = [&](int slot, int t) {       // t: this thread's token of that tile
+      bar_sync(kDone + slot, kScanThreads);
+      if (t < stop) {
+        float o[4];
+        f2 v[2];
+        ld2(&sy[slot][row][4 * sub], v);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          f2 y = fma2(Dv[j], px2[j], v[j]);
+          if (gated) y = mul2(y, mul2(pz2[j], vsigmoid<2>(Fv<2>{{pz2[j]}}).p[0]));
+          const float2 r = unpack(y);
+          o[2 * j] = t < end ? r.x : 0.0f;
+          o[2 * j + 1] = t < end ? r.y : 0.0f;
+        }
+        store_row<T, 4, VEC>(py, c, E, o);
+      }
+      py += (int64_t)kTile * E;
+    };
+    if (begin < end) fetch();
+    int at = begin + row;                      // token of the tile being staged
+    for (int t0 = begin; t0 < end; t0 += kTile) {
+      f2 xs[2], zs[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        xs[j] = pack(rx.get(2 * j), rx.get(2 * j + 1));
+        zs[j] = gated ? pack(rz.get(2 * j), rz.get(2 * j + 1)) : f2{0ull};
+        f2 d = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]), u;
+        if (a.softplus) d = softplus2(d, u);
+        if (at >= end) d = f2{0ull};
+        const float2 dv = unpack(d), uv = unpack(mul2(d, xs[j]));
+        st4(&sd[slot][row][4 * sub + 2 * j], make_float4(dv.x, dv.x, dv.y, dv.y));
+        st4(&su[slot][row][4 * sub + 2 * j], make_float4(uv.x, uv.x, uv.y, uv.y));
+      }
+      st4(&sbc[slot][row][4 * sub], make_float4(rb.get(0), rb.get(1), rb.get(2), rb.get(3)));
+      bar_arrive(kFull + slot, kScanThreads);
+      if (t0 + kTile < end) fetch();
+      if (t0 > begin) finish(slot ^ 1, at - kTile);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        px2[j] = xs[j];
+        pz2[j] = zs[j];
+      }
+      at += kTile;
+      slot ^= 1;
+    }
+    if (begin < end) finish(slot ^ 1, at - kTile);
+    const float zero[4] = {};
+    for (; at < stop; at += kTile) {           // tiles wholly behind the row's end
+      store_row<T, 4, VEC>(py, c, E, zero);
+      py += (int64_t)kTile * E;
+    }
+  }
+}
+
+// Only a part's end state (from zero) and sum of d.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kSsmThreads) k_ssm_ends(const boa_ssm_args a, const SsmPlan p,
+                                                          float* __restrict__ ends, float* __restrict__ dsum) {
+  __shared__ __align__(16) float sd[kTile][kPitch], su[kTile][kPitch], sb[kTile][kN];
+  const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
+  const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels, nparts = p.parts - 1;
+  const int part = (blockIdx.x / p.cblocks) % nparts, b = blockIdx.x / p.cblocks / nparts;
+  const int e = e0 + ch;
+  const bool on = e < E;
+  const int begin = part * p.part, end = min(min(begin + p.part, a.length), row_len(a, b));
+  const int64_t slot = ((int64_t)b * p.parts + part) * E + e;
+  const int row = tid >> 3, sub = tid & 7, c = e0 + 4 * sub;
+  int t = begin + row;
+  const T* px = (const T*)a.x + b * a.x_bs + t * a.x_ts + c;
+  const T* pd = (const T*)a.dt + b * a.dt_bs + t * a.dt_ts + c;
+  const T* pb = (const T*)a.B + b * a.B_bs + t * a.B_ts + 4 * sub;   // threads with sub < 4
+  f2 bias[2], A2[2], h[2] = {f2{0ull}, f2{0ull}};
+  load_pairs(a.dt_bias, c, E, bias);
+  {
+    float v[kQ];
+#pragma unroll
+    for (int j = 0; j < kQ; ++j) v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+    A2[0] = pack(v[0], v[1]);
+    A2[1] = pack(v[2], v[3]);
+  }
+  float total = 0.0f;
+  Row<T, 4, VEC> rx, rd, rb;
+  auto fetch = [&]() {
+    const bool live = t < end;
+    rx.load(px, c, E, live);
+    rd.load(pd, c, E, live);
+    rb.load(pb, 0, 4, live && sub < 4);
+    px += kTile * a.x_ts;
+    pd += kTile * a.dt_ts;
+    pb += kTile * a.B_ts;
+  };
+  if (begin < end) fetch();
+  for (int t0 = begin; t0 < end; t0 += kTile) {
+    f2 d[2], u[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      d[j] = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]);
+      if (a.softplus) d[j] = softplus2(d[j], u[j]);
+      if (t >= end) d[j] = f2{0ull};
+      u[j] = mul2(d[j], pack(rx.get(2 * j), rx.get(2 * j + 1)));
+    }
+    st2(&sd[row][4 * sub], d);
+    st2(&su[row][4 * sub], u);
+    if (sub < 4) st4(&sb[row][4 * sub], make_float4(rb.get(0), rb.get(1), rb.get(2), rb.get(3)));
+    t += kTile;
+    __syncthreads();
+    if (t0 + kTile < end) fetch();
+#pragma unroll
+    for (int i = 0; i < kTile; ++i) {
+      const float dk = sd[i][ch], uk = su[i][ch];
+      const f2 dd = pack(dk, dk), uu = pack(uk, uk);
+      const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sb[i][kQ * q]);
+      h[0] = fma2(ex2_2(mul2(dd, A2[0])), h[0], mul2(uu, f2{B.x}));
+      h[1] = fma2(ex2_2(mul2(dd, A2[1])), h[1], mul2(uu, f2{B.y}));
+      total += dk;
+    }
+    __syncthreads();
+  }
+  if (on) {
+    *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(h[0].v, h[1].v);
+    if (q == 0) dsum[slot] = total;
   }
 }
 
@@ -297,7 +388,7 @@ static __global__ void __launch_bounds__(128) k_ssm_join(int64_t n, int E, int p
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_args a, const SsmPlan p,
                                                                float* __restrict__ ends, float* __restrict__ dsum) {
-  __shared__ __align__(16) f2 sd[kTile][kCh], sg[kTile][kCh];
+  __shared__ __align__(16) float sd[kTile][kPitch], sg[kTile][kPitch];
   __shared__ __align__(16) float sc[kTile][kN];
   const int tid = threadIdx.x, lane = tid & 31, q = lane_q(lane), ch = (tid >> 5) * 8 + lane_ch(lane);
   const int e0 = (blockIdx.x % p.cblocks) * kCh, E = a.channels;
@@ -323,7 +414,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
     A2[0] = pack(v[0], v[1]);
     A2[1] = pack(v[2], v[3]);
   }
-  f2 total{0ull};
+  float total = 0.0f;
   Row<T, 4, VEC> rg, rd, rz, rc;
   auto fetch = [&]() {
     const bool live = t < end;
@@ -338,19 +429,21 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
   };
   if (tiles) fetch();
   for (int k = tiles - 1; k >= 0; --k) {
+    f2 d[2], g[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      f2 d = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]), u, g = pack(rg.get(2 * j), rg.get(2 * j + 1));
-      if (a.softplus) d = softplus2(d, u);
-      if (t >= end) d = f2{0ull};
+      f2 u;
+      d[j] = add2(pack(rd.get(2 * j), rd.get(2 * j + 1)), bias[j]);
+      g[j] = pack(rg.get(2 * j), rg.get(2 * j + 1));
+      if (a.softplus) d[j] = softplus2(d[j], u);
+      if (t >= end) d[j] = f2{0ull};
       if (gated) {
         const f2 z = pack(rz.get(2 * j), rz.get(2 * j + 1));
-        g = mul2(g, mul2(z, vsigmoid<2>(Fv<2>{{z}}).p[0]));
+        g[j] = mul2(g[j], mul2(z, vsigmoid<2>(Fv<2>{{z}}).p[0]));
       }
-      const float2 dv = unpack(d), gv = unpack(g);
-      *reinterpret_cast<float4*>(&sd[row][4 * sub + 2 * j]) = make_float4(dv.x, dv.x, dv.y, dv.y);
-      *reinterpret_cast<float4*>(&sg[row][4 * sub + 2 * j]) = make_float4(gv.x, gv.x, gv.y, gv.y);
     }
+    st2(&sd[row][4 * sub], d);
+    st2(&sg[row][4 * sub], g);
     if (sub < 4)
       *reinterpret_cast<float4*>(&sc[row][4 * sub]) = make_float4(rc.get(0), rc.get(1), rc.get(2), rc.get(3));
     t -= kTile;
@@ -358,17 +451,18 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
     if (k > 0) fetch();
 #pragma unroll
     for (int i = kTile - 1; i >= 0; --i) {
-      const f2 dd = sd[i][ch], gg = sg[i][ch];
+      const float dk = sd[i][ch], gk = sg[i][ch];
+      const f2 dd = pack(dk, dk), gg = pack(gk, gk);
       const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sc[i][kQ * q]);
       g2[0] = mul2(ex2_2(mul2(dd, A2[0])), fma2(f2{C.x}, gg, g2[0]));
       g2[1] = mul2(ex2_2(mul2(dd, A2[1])), fma2(f2{C.y}, gg, g2[1]));
-      total = add2(total, dd);
+      total += dk;
     }
     __syncthreads();
   }
   if (on) {
     *reinterpret_cast<ulonglong2*>(ends + slot * kN + kQ * q) = make_ulonglong2(g2[0].v, g2[1].v);
-    if (q == 0) dsum[slot] = unpack(total).x;
+    if (q == 0) dsum[slot] = total;
   }
 }
 
@@ -395,17 +489,6 @@ struct BackSmem {
   __host__ __device__ static constexpr int floats(int passes) { return carry + passes * kBackCh * per_channel; }
 };
 static_assert(BackSmem::floats(kPasses) * 4 <= 227 * 1024, "shared memory of a block");
-
-__device__ __forceinline__ void bar_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(int id, int threads) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-enum { kFull = 1, kDone = 3, kScanOnly = 5 };          // barrier ids; kFull and kDone one per slot
-
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ void st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 
 // A block takes one part of a row and up to 512 channels, tile by tile (8
 // tokens) from the end, 64 channels a pass.  The last four warps stage a pass
@@ -918,11 +1001,11 @@ static int ssm_forward_t(const boa_ssm_args& a, cudaStream_t s) {
   float* ends = (float*)a.workspace;
   float* dsum = ends + (size_t)a.batch * p.parts * a.channels * kN;
   if (p.parts > 1) {
-    k_ssm<T, true, VEC><<<(unsigned)((int64_t)p.cblocks * (p.parts - 1) * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
+    k_ssm_ends<T, VEC><<<(unsigned)((int64_t)p.cblocks * (p.parts - 1) * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
     const int64_t n = (int64_t)a.batch * a.channels * kN;
     k_ssm_join<<<(unsigned)((n + 127) / 128), 128, 0, s>>>(n, a.channels, p.parts, a.A, a.state, ends, dsum, false);
   }
-  k_ssm<T, false, VEC><<<(unsigned)((int64_t)p.cblocks * p.parts * a.batch), kSsmThreads, 0, s>>>(a, p, ends, dsum);
+  k_ssm<T, VEC><<<(unsigned)((int64_t)p.cblocks * p.parts * a.batch), kScanThreads, 0, s>>>(a, p, ends);
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
 }
