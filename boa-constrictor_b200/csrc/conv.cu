@@ -355,7 +355,7 @@ static ConvRuns conv_runs(const boa_conv_args& a, int V, int64_t want) {
 // Forward: a few waves of blocks, so that the last one is short.  Backward: about
 // four rounds of the blocks that the SMs hold (512 threads each, by registers).
 static ConvRuns runs_forward(const boa_conv_args& a, int V) { return conv_runs(a, V, 148LL * 2048); }
-static ConvRuns runs_backward(const boa_conv_args& a, int V) { return conv_runs(a, V, 148LL * 1500); }
+static ConvRuns runs_backward(const boa_conv_args& a, int V) { return conv_runs(a, V, 148LL * 800); }
 
 // Whether every row of every tensor starts on a vector of kConvVec elements.
 static bool conv_vec(const boa_conv_args& a, bool backward, bool step) {
@@ -401,7 +401,7 @@ static int conv_launch(const boa_conv_args& a, int what, cudaStream_t s) {
       BOA_CUDA(cudaFuncSetAttribute(k_conv_backward<T, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     k_conv_backward<T, V, K><<<(unsigned)(blocks * r.group_blocks), kConvThreads, smem, s>>>(a, r, parts, blocks);
     const int cols = (K + 1) * a.channels;
-    k_sum_parts<<<(cols + 31) / 32, 512, 0, s>>>(parts, blocks, cols, K * a.channels, cols, a.dweight, a.dbias,
+    k_sum_parts<<<(cols + 31) / 32, 1024, 0, s>>>(parts, blocks, cols, K * a.channels, cols, a.dweight, a.dbias,
                                                 nullptr);
   }
   BOA_CUDA(cudaGetLastError());

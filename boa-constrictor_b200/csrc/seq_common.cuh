@@ -348,25 +348,25 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // Sum of n_parts partial rows: column c of the result is sum_p parts[p * cols + c],
-// in a fixed order.  A block owns 32 columns; its 16 warps take the rows in turn
+// in a fixed order.  A block owns 32 columns; its 32 warps take the rows in turn
 // and are joined in shared memory.  Columns [0, s1) go to o1, [s1, s2) to o2 and
 // the rest to o3 (NULL: dropped), so one launch finishes up to three gradients.
-static __global__ void __launch_bounds__(512) k_sum_parts(const float* __restrict__ parts, int64_t n_parts, int cols,
+static __global__ void __launch_bounds__(1024) k_sum_parts(const float* __restrict__ parts, int64_t n_parts, int cols,
                                                           int s1, int s2, float* __restrict__ o1,
                                                           float* __restrict__ o2, float* __restrict__ o3) {
-  __shared__ float red[16][33];
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (c < cols)
-#pragma unroll 4
-    for (int64_t p = w; p < n_parts; p += 16) s += parts[p * cols + c];
+#pragma unroll 8
+    for (int64_t p = w; p < n_parts; p += 32) s += parts[p * cols + c];
   red[w][lane] = s;
   __syncthreads();
   if (w == 0 && c < cols) {
     float t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += red[i][lane];
+    for (int i = 0; i < 32; ++i) t += red[i][lane];
     if (c < s1) o1[c] = t;
     else if (c < s2) { if (o2) o2[c - s1] = t; }
     else if (o3) o3[c - s2] = t;

@@ -1044,7 +1044,7 @@ static int ssm_backward_t(const boa_ssm_args& a, cudaStream_t s) {
   if (n > 0 && groups > 1)
     k_ssm_bc<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(rows, groups, bc, (T*)a.dB, (T*)a.dC);
   const int cols = a.channels * (kN + 2);
-  k_sum_parts<<<(cols + 31) / 32, 512, 0, s>>>(params, (int64_t)a.batch * p.parts, cols, a.channels * kN,
+  k_sum_parts<<<(cols + 31) / 32, 1024, 0, s>>>(params, (int64_t)a.batch * p.parts, cols, a.channels * kN,
                                               a.channels * (kN + 1), a.dA, a.dD, a.ddt_bias);
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
