@@ -154,7 +154,9 @@ def test_causal_conv_continues_over_pieces():
 
 
 @pytest.mark.parametrize("B,E,K,kind,silu", [(1, 1, 4, F32, True), (16, 128, 4, F32, True), (33, 515, 3, BF16, True),
-                                             (7, 64, 2, F16, False), (1000, 512, 4, BF16, True)])
+                                             (7, 64, 2, F16, False), (1000, 512, 4, BF16, True),
+                                             # so many that a thread takes several streams
+                                             (2401, 512, 4, BF16, True), (613, 515, 4, F32, True)])
 def test_causal_conv_step(B, E, K, kind, silu):
     x, w, b, s, _, _ = _conv_case(B, 5, E, K, kind, E, True)
     wide = torch.empty(B, 5, 2 * E, dtype=kind).normal_().cuda()
@@ -280,7 +282,9 @@ def test_ssm_scan_decays_that_vanish_or_stay():
     _scan_check(c, None, got)
 
 
-@pytest.mark.parametrize("B,E,kind", [(1, 1, F32), (16, 128, F32), (9, 515, BF16), (40, 96, F16)])
+@pytest.mark.parametrize("B,E,kind", [(1, 1, F32), (16, 128, F32), (9, 515, BF16), (40, 96, F16),
+                                      # so many that a thread takes several streams; the last group is not whole
+                                      (613, 515, BF16), (601, 512, F32), (1187, 256, F16)])
 def test_ssm_step(B, E, kind):
     """Steps from a state against 64 bits, and the state they leave."""
     c = _scan_case(B, 6, E, kind, E)
