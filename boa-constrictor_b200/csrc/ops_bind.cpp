@@ -35,7 +35,11 @@ struct Refused {            // bad arguments: ValueError, or RuntimeError for th
 };
 struct Failed : std::runtime_error {   // an error code of the library: BoaError (RuntimeError inside backward)
   int code;
-  Failed(int c, const std::string& what) : std::runtime_error(what), code(c) {}
+  std::string plain;                   // BoaError adds the code itself
+  Failed(int c, const std::string& p) : std::runtime_error(with_code(c, p)), code(c), plain(p) {}
+  static std::string with_code(int c, const std::string& p) {
+    return "[boa_b200 error " + std::to_string(c) + "] " + p;
+  }
 };
 
 void put(std::ostringstream& s, const char* v) { s << v; }
@@ -113,7 +117,7 @@ void need_api() {
 }
 
 void check(int rc, const char* name) {
-  if (rc != BOA_OK) throw Failed(rc, text("[boa_b200 error ", rc, "] ", name, ": ", api.last_error()));
+  if (rc != BOA_OK) throw Failed(rc, text(name, ": ", api.last_error()));
 }
 
 // ---------------------------------------------------------------- arguments
@@ -123,6 +127,8 @@ int dtype_code(at::ScalarType t) {
 void check_kind(const char* who, const Tensor& x) {
   if (dtype_code(x.scalar_type()) < 0)
     refuse(text(who, ": x must be float32, bfloat16 or float16, not ", x.scalar_type()));
+  for (const int64_t n : x.sizes())      // the entry points take 32-bit sizes
+    if (n > INT32_MAX) refuse(text(who, ": every size of x must be below 2^31, got ", x.sizes()));
 }
 void check_shape(const char* who, const char* name, const Tensor& t, at::IntArrayRef want) {
   if (t.sizes() != want) refuse(text(who, ": ", name, " must have shape ", want, ", got ", t.sizes()));
@@ -365,8 +371,8 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   boa_conv_args a = conv_args(x, w, b, silu, Tensor(), Tensor());
   a.y = ptr(y);
   a.state_out = ptr(state);
-  check(api.causal_conv_step(&a, stream_of(x)), "boa_causal_conv_step");
   state.unsafeGetTensorImpl()->bump_version();
+  check(api.causal_conv_step(&a, stream_of(x)), "boa_causal_conv_step");
   return y;
 }
 
@@ -539,8 +545,8 @@ Tensor ssm_step(SsmIn i, bool softplus) {
   a.state = nullptr;
   a.y = ptr(y);
   a.state_out = fptr(i.state);
-  check(api.ssm_step(&a, stream_of(i.x)), "boa_ssm_step");
   i.state.unsafeGetTensorImpl()->bump_version();
+  check(api.ssm_step(&a, stream_of(i.x)), "boa_ssm_step");
   return y;
 }
 
@@ -583,7 +589,7 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F f) {
     PyErr_SetString(r.type, r.text.c_str());
     return nullptr;
   } catch (const Failed& e) {
-    if (PyObject* v = PyObject_CallFunction(boa_error, "is", e.code, e.what())) {
+    if (PyObject* v = PyObject_CallFunction(boa_error, "is", e.code, e.plain.c_str())) {
       PyErr_SetObject(boa_error, v);
       Py_DECREF(v);
     }

@@ -456,6 +456,58 @@ def test_captured_and_replayed():
             assert torch.equal(o, want[i][k]), (i, j, k)
 
 
+def test_empty_sequences_backward():
+    """No tokens: the states' gradients pass through, the parameters' are zero.  No rows: all gradients are zero."""
+    ops = _ops()
+    c = _scan_case(2, 0, 24, F32, 70)
+    got, _ = _scan_grads(c, None)
+    assert torch.equal(got["state"], c["state"].cuda()) and torch.equal(got["dstate"], c["dout"].cuda())
+    assert all((got[k] == 0).all() for k in ("dA", "dD", "dbias"))
+    x, w, b, s, dy, ds = _conv_case(2, 0, 8, 4, F32, 71, True)
+    xs, ws, bs, ss = _cuda(x, True), _cuda(w, True), _cuda(b, True), _cuda(s, True)
+    y, out = ops.causal_conv(xs, ws, bs, state=ss, return_state=True)
+    g = torch.autograd.grad((y, out), (ws, bs, ss), (dy.cuda(), ds.cuda()))
+    assert torch.equal(out, s.cuda()) and (g[0] == 0).all() and (g[1] == 0).all() and torch.equal(g[2], ds.cuda())
+    c = _scan_case(0, 5, 24, F32, 72)
+    got, _ = _scan_grads(c, None)
+    assert all((got[k] == 0).all() for k in ("dA", "dD", "dbias"))
+    x, w, b, _, dy, _ = _conv_case(0, 5, 8, 4, F32, 73, False)
+    ws = _cuda(w, True)
+    assert (torch.autograd.grad(ops.causal_conv(_cuda(x), ws).sum(), ws)[0] == 0).all()
+
+
+def test_without_bias_backward():
+    """The gradients without a bias are those with a bias of zero."""
+    ops = _ops()
+    x, w, _, _, dy, _ = _conv_case(2, 40, 24, 4, F32, 74, False)
+    zero = torch.zeros(24)
+    a, b = _cuda(x, True), _cuda(w, True)
+    one = torch.autograd.grad(ops.causal_conv(a, b), (a, b), dy.cuda())
+    two = torch.autograd.grad(ops.causal_conv(a, b, _cuda(zero)), (a, b), dy.cuda())
+    assert _equal(one, two)
+    v = _cuda(1 + 0.1 * torch.randn(24, generator=_gen(5)), True)
+    one = torch.autograd.grad(ops.layer_norm(a, v), (a, v), dy.cuda())
+    two = torch.autograd.grad(ops.layer_norm(a, v, _cuda(zero)), (a, v), dy.cuda())
+    assert _equal(one, two)
+
+
+def test_library_errors_and_inference_mode():
+    from boa_b200 import _native as _n
+    ops = _ops()
+    with pytest.raises(_n.BoaError, match="width must be at most 8192") as e:
+        ops.layer_norm(torch.zeros(1, 8193, device="cuda"), torch.ones(8193, device="cuda"))
+    assert e.value.code == _n.BOA_ERR_UNSUPPORTED
+    with torch.inference_mode():
+        st = torch.zeros(2, 3, 8, device="cuda")
+        x = torch.ones(2, 8, device="cuda")
+        ops.causal_conv_step(x, st, torch.ones(8, 4, device="cuda"))
+    assert torch.equal(st[:, 2], x) and (st[:, :2] == 0).all()
+    # its own state again from outside is refused before anything is written
+    with pytest.raises(RuntimeError, match="[Ii]nference"):
+        ops.causal_conv_step(x, st, torch.ones(8, 4, device="cuda"))
+    assert (st[:, :2] == 0).all()
+
+
 def test_second_derivatives_are_refused():
     ops = _ops()
     x = torch.randn(4, 16, device="cuda", requires_grad=True)

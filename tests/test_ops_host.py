@@ -99,6 +99,23 @@ def test_ssm_state_refusals():
             ops.ssm_step(*s)
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    wide = torch.zeros(1, 1, 1).expand(2 ** 31, 1, 1)
+    with pytest.raises(ValueError, match="below 2"):
+        ops.causal_conv(wide, torch.zeros(1, 4))
+    with pytest.raises(ValueError, match="below 2"):
+        ops.layer_norm(wide[:, 0, 0], torch.zeros(1))
+    with pytest.raises(ValueError, match="below 2"):
+        ops.ssm_scan(wide, wide, torch.zeros(1, 16), wide.expand(-1, -1, 16), wide.expand(-1, -1, 16))
+
+
+def test_not_a_tensor():
+    with pytest.raises(TypeError, match="weight must be a tensor"):
+        ops.layer_norm(torch.zeros(2, 8), None)
+    with pytest.raises(TypeError, match="x must be a tensor"):
+        ops.causal_conv([1.0], torch.zeros(8, 4))
+
+
 def test_struct_layout_matches_header(tmp_path):
     """Field offsets and sizes of the ctypes structs are the C compiler's."""
     src = ["#include <stdio.h>", "#include <stddef.h>", '#include "boa_b200.h"', "int main(void) {"]
