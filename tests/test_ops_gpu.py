@@ -210,7 +210,9 @@ def _scan_check(c, lens, got, plus=True):
 
 @pytest.mark.parametrize("B,L,E,lens", [
     (1, 1, 1, None), (2, 1, 33, (0, 1)), (1, 7, 32, None), (2, 8, 31, (8, 3)), (3, 17, 128, (17, 0, 16)),
-    (1, 64, 40, None), (2, 130, 65, (129, 130)), (1, 300, 288, None), (2, 65, 520, (1, 64)), (5, 33, 16, (-1, 99, 32, 8, 9))])
+    (1, 64, 40, None), (2, 130, 65, (129, 130)), (1, 300, 288, None), (2, 65, 520, (1, 64)), (5, 33, 16, (-1, 99, 32, 8, 9)),
+    # rows enough that neither direction splits the length
+    (1300, 9, 8, None), (300, 20, 40, (20, 0, 7) * 100)])
 @pytest.mark.parametrize("kind,gate,state", [(F32, True, True), (F32, False, False), (BF16, True, True),
                                              (F16, True, False)])
 def test_ssm_scan(B, L, E, lens, kind, gate, state):
@@ -368,6 +370,27 @@ def test_strides_and_broadcast_inputs():
     t = torch.zeros(3, 21, 41, device="cuda")
     t[..., 3:37] = x
     assert torch.equal(ops.causal_conv(t[..., 3:37], w), ops.causal_conv(x, w))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^31 elements apart, and a result of more than 2^31 elements."""
+    ops = _ops()
+    store = torch.zeros(2 ** 31 + 4096, dtype=BF16, device="cuda")
+    far = store.as_strided((2, 40, 24), (2 ** 31, 24, 1))
+    g = _gen(80)
+    near = torch.randn(2, 40, 24, generator=g).to(BF16).cuda()
+    far.copy_(near)
+    w = torch.randn(24, 4, generator=g).cuda()
+    assert torch.equal(ops.causal_conv(far, w), ops.causal_conv(near, w))
+    c = _scan_case(2, 40, 24, BF16, 81)
+    d = {k: _cuda(c[k]) for k in ("dt", "A", "B", "C", "D", "z", "bias")}
+    f = lambda x: ops.ssm_scan(x, d["dt"], d["A"], d["B"], d["C"], d["D"], d["z"], d["bias"])  # noqa: E731
+    assert torch.equal(f(far), f(near))
+    del store, far
+    x = torch.randn(1, 2048, device="cuda", dtype=BF16).expand(2 ** 20 + 3, 2048)
+    p = torch.ones(2048, device="cuda")
+    y = ops.layer_norm(x, p)
+    assert torch.equal(y[-1], y[0]) and torch.equal(y[2 ** 19], y[0]) and torch.equal(y[:1], ops.layer_norm(x[:1], p))
 
 
 def test_same_tensor_twice():
