@@ -91,14 +91,6 @@ struct Words {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void load_f(const T* p, float (&out)[V]) {
-  Words<T, V> r;
-  r.load(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = r.get(i);
-}
-
-template <typename T, int V>
 __device__ __forceinline__ void store_f(T* p, const float (&in)[V]) {
   Words<T, V> r;
   r.set(in);

@@ -288,7 +288,7 @@ BOA_API int boa_layer_norm_backward(int64_t rows, int width, int dtype, const vo
  * row's valid length, clamped to [0, length]; positions behind it are not read
  * and their y and dx are zero.  The fields behind `state_out` are the backward
  * call's: dy, dstate_out (NULL: zeros) in; dx, dweight, dbias (NULL when bias
- * is), dstate (may be NULL) out. */
+ * is), dstate (may be NULL) out.  weight is 16-byte aligned. */
 typedef struct boa_conv_args {
   int32_t dtype, batch, length, channels, width, silu, device, reserved;
   const void* x;
@@ -326,7 +326,8 @@ BOA_API int boa_causal_conv_step(const boa_conv_args* a, void* stream);
  * boa_conv_args.  `checkpoints` (NULL unless a backward call follows;
  * boa_ssm_checkpoint_bytes) receives the states the backward call restarts
  * from.  The fields behind `checkpoints` are the backward call's; dz, dD,
- * ddt_bias, dstate may be NULL where their input is. */
+ * ddt_bias, dstate may be NULL where their input is.  workspace and
+ * checkpoints are 16-byte aligned, and so are A and the state of a step. */
 typedef struct boa_ssm_args {
   int32_t dtype, batch, length, channels, states, softplus, device, reserved;
   const void* x;
