@@ -338,6 +338,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_ends(const boa_ssm_args a, 
     t += kTile;
     __syncthreads();
     if (t0 + kTile < end) fetch();
+    float tile = 0.0f;
 #pragma unroll
     for (int i = 0; i < kTile; ++i) {
       const float dk = sd[i][ch], uk = su[i][ch];
@@ -345,8 +346,9 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_ends(const boa_ssm_args a, 
       const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(&sb[i][kQ * q]);
       h[0] = fma2(ex2_2(mul2(dd, A2[0])), h[0], mul2(uu, f2{B.x}));
       h[1] = fma2(ex2_2(mul2(dd, A2[1])), h[1], mul2(uu, f2{B.y}));
-      total += dk;
+      tile += dk;
     }
+    total += tile;   // by tiles: a part's sum then passes tens of roundings, not one a token
     __syncthreads();
   }
   if (on) {
@@ -455,6 +457,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
     t -= kTile;
     __syncthreads();
     if (k > 0) fetch();
+    float tile = 0.0f;
 #pragma unroll
     for (int i = kTile - 1; i >= 0; --i) {
       const float dk = sd[i][ch], gk = sg[i][ch];
@@ -462,8 +465,9 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
       const ulonglong2 C = *reinterpret_cast<const ulonglong2*>(&sc[i][kQ * q]);
       g2[0] = mul2(ex2_2(mul2(dd, A2[0])), fma2(f2{C.x}, gg, g2[0]));
       g2[1] = mul2(ex2_2(mul2(dd, A2[1])), fma2(f2{C.y}, gg, g2[1]));
-      total += dk;
+      tile += dk;
     }
+    total += tile;   // by tiles: a part's sum then passes tens of roundings, not one a token
     __syncthreads();
   }
   if (on) {
