@@ -8,9 +8,10 @@ kernels of libboa_b200.so (``boa_layer_norm``, ``boa_causal_conv``,
 * ``ssm_scan(x, dt, A, B, C, D, z, dt_bias, ...)``      the mixer's selective state space scan
 * ``ssm_step(x, dt, state, A, B, C, D, z, dt_bias)``    the same for one token per stream
 
-The sequence forms are differentiable in every floating argument (once: there
-is no second derivative, and a backward pass with ``create_graph`` is refused);
-the step forms update their state in place and are for inference.
+The sequence forms are differentiable in every floating argument (in reverse
+mode and once: a backward pass with ``create_graph`` and inputs with a
+forward-mode tangent are refused); the step forms update their state in place
+and are for inference.
 
 Sequences are ``[batch, length, channels]``.  Activations of one call share one
 type (float32, bfloat16 or float16); their rows may be strided (a slice of a

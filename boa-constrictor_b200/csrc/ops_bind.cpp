@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -167,6 +168,15 @@ Tensor int_lens(const char* who, const Tensor& lens, int64_t batch, int64_t leng
   check_shape(who, "lens", lens, {batch});
   return (lens.scalar_type() == at::kInt ? lens : lens.clamp(0, length).to(at::kInt)).contiguous();
 }
+// A tangent (torch.autograd.forward_ad) is no requires_grad: without this the
+// raw call would drop it, and a dropped tangent reads as a derivative of zero.
+void reverse_mode_only(const char* who, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(/*level=*/0).defined())
+      throw Refused{PyExc_RuntimeError,
+                    text(who, " has no forward-mode derivative: take derivatives with backward() or torch.autograd.grad")};
+}
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -190,9 +200,15 @@ using Opt = std::optional<Tensor>;
 Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 Tensor val(const Opt& o) { return o.has_value() ? *o : Tensor(); }
 
-void first_order_only(const char* who) {
+// For a backward call with the incoming gradients `up` and the saved inputs.
+void first_order_only(const char* who, const variable_list& up, const variable_list& saved) {
   if (at::GradMode::is_enabled())
     throw std::runtime_error(text(who, " has no second derivative: call backward without create_graph"));
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const variable_list* v : {&up, &saved})
+    for (const Tensor& t : *v)
+      if (t.defined() && t._fw_grad(/*level=*/0).defined())
+        throw std::runtime_error(text(who, " has no second derivative: its backward takes no forward-mode tangents"));
 }
 // dy as the kernels read it; zeros when only the final state was used
 Tensor upstream(const Tensor& dy, const Tensor& x) {
@@ -220,8 +236,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list up) {
-    first_order_only("layer_norm");
     const variable_list s = ctx->get_saved_variables();
+    first_order_only("layer_norm", up, s);
     const Tensor &x = s[0], &w = s[1], &stats = s[2];
     OnDevice on(x);
     const Tensor dy = rows(up[0]);
@@ -245,6 +261,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
   const int64_t width = x.size(-1);
   check_shape(who, "weight", weight, {width});
   if (bias.defined()) check_shape(who, "bias", bias, {width});
+  reverse_mode_only(who, {&x, &weight, &bias});
   check_device(who, x, {&weight, &bias});
   const Tensor w = param(weight), b = param(bias);
   const Tensor flat = rows(x.dim() == 2 ? x : x.reshape({-1, width}));
@@ -297,8 +314,8 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     return conv_forward(x, w, b, state, lens, silu, return_state);
   }
   static variable_list backward(AutogradContext* ctx, variable_list up) {
-    first_order_only("causal_conv");
     const variable_list s = ctx->get_saved_variables();
+    first_order_only("causal_conv", up, s);
     const Tensor &x = s[0], &w = s[1], &b = s[2], &state = s[3];
     OnDevice on(x);
     boa_conv_args a = conv_args(x, w, b, ctx->saved_data["silu"].toBool(), state, s[4]);
@@ -343,6 +360,7 @@ variable_list causal_conv(const Tensor& x_, const Tensor& weight, const Tensor& 
     check_same(who, "state", x_, state_);
   }
   const Tensor lens = int_lens(who, lens_, n, length);
+  reverse_mode_only(who, {&x_, &weight, &bias, &state_});
   check_device(who, x_, {&w, &bias, &state_, &lens});
   w = param(w);
   const Tensor b = param(bias), x = rows(x_), state = state_.defined() ? state_.contiguous() : state_;
@@ -360,6 +378,7 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   check_shape(who, "state", state, {n, w.size(1) - 1, e});
   check_same(who, "state", x_, state);
   if (!state.is_contiguous()) refuse(text(who, ": state is updated in place and must be contiguous"));
+  reverse_mode_only(who, {&x_, &state, &weight, &bias});
   check_device(who, x_, {&state, &w, &bias});
   if (wants_grad({&x_, &state, &w, &bias}))
     throw Refused{PyExc_RuntimeError,
@@ -446,8 +465,8 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list up) {
-    first_order_only("ssm_scan");
     const variable_list s = ctx->get_saved_variables();
+    first_order_only("ssm_scan", up, s);
     const SsmIn i{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9]};
     const Tensor& x = i.x;
     OnDevice on(x);
@@ -521,6 +540,7 @@ variable_list ssm_scan(SsmIn i, bool softplus, bool return_state) {
   const char* who = "ssm_scan";
   ssm_check(who, i, 3);
   i.lens = int_lens(who, i.lens, i.x.size(0), i.x.size(1));
+  reverse_mode_only(who, {&i.x, &i.dt, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias, &i.state});
   check_device(who, i.x, {&i.dt, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias, &i.state, &i.lens});
   ssm_prepare(i);
   i.state = param(i.state);
@@ -535,6 +555,7 @@ Tensor ssm_step(SsmIn i, bool softplus) {
   ssm_check(who, i, 2);
   if (!i.state.is_contiguous() || misaligned(i.state))
     refuse(text(who, ": state is updated in place and must be contiguous and 16-byte aligned"));
+  reverse_mode_only(who, {&i.x, &i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias});
   check_device(who, i.x, {&i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias});
   if (wants_grad({&i.x, &i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias}))
     throw Refused{PyExc_RuntimeError, text(who, " has no gradient: call it under torch.no_grad(), or use ssm_scan")};
