@@ -11,7 +11,7 @@ kernels of libboa_b200.so (``boa_layer_norm``, ``boa_causal_conv``,
 The sequence forms are differentiable in every floating argument (in reverse
 mode and once: a backward pass with ``create_graph`` and inputs with a
 forward-mode tangent are refused); the step forms update their state in place
-and are for inference.
+and are for inference.  ``torch.jit.trace`` is refused too.
 
 Sequences are ``[batch, length, channels]``.  Activations of one call share one
 type (float32, bfloat16 or float16); their rows may be strided (a slice of a

@@ -14,6 +14,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <sstream>
 #include <stdexcept>
@@ -177,6 +178,11 @@ void reverse_mode_only(const char* who, std::initializer_list<const Tensor*> ts)
       throw Refused{PyExc_RuntimeError,
                     text(who, " has no forward-mode derivative: take derivatives with backward() or torch.autograd.grad")};
 }
+// torch.jit.trace cannot see into a call: it would record its result as a constant.
+void no_tracing(const char* who) {
+  if (torch::jit::tracer::isTracing())
+    throw Refused{PyExc_RuntimeError, text(who, " cannot be traced: its result would become a constant")};
+}
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -261,6 +267,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, dou
   const int64_t width = x.size(-1);
   check_shape(who, "weight", weight, {width});
   if (bias.defined()) check_shape(who, "bias", bias, {width});
+  no_tracing(who);
   reverse_mode_only(who, {&x, &weight, &bias});
   check_device(who, x, {&weight, &bias});
   const Tensor w = param(weight), b = param(bias);
@@ -360,6 +367,7 @@ variable_list causal_conv(const Tensor& x_, const Tensor& weight, const Tensor& 
     check_same(who, "state", x_, state_);
   }
   const Tensor lens = int_lens(who, lens_, n, length);
+  no_tracing(who);
   reverse_mode_only(who, {&x_, &weight, &bias, &state_});
   check_device(who, x_, {&w, &bias, &state_, &lens});
   w = param(w);
@@ -378,6 +386,7 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   check_shape(who, "state", state, {n, w.size(1) - 1, e});
   check_same(who, "state", x_, state);
   if (!state.is_contiguous()) refuse(text(who, ": state is updated in place and must be contiguous"));
+  no_tracing(who);
   reverse_mode_only(who, {&x_, &state, &weight, &bias});
   check_device(who, x_, {&state, &w, &bias});
   if (wants_grad({&x_, &state, &w, &bias}))
@@ -540,6 +549,7 @@ variable_list ssm_scan(SsmIn i, bool softplus, bool return_state) {
   const char* who = "ssm_scan";
   ssm_check(who, i, 3);
   i.lens = int_lens(who, i.lens, i.x.size(0), i.x.size(1));
+  no_tracing(who);
   reverse_mode_only(who, {&i.x, &i.dt, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias, &i.state});
   check_device(who, i.x, {&i.dt, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias, &i.state, &i.lens});
   ssm_prepare(i);
@@ -555,6 +565,7 @@ Tensor ssm_step(SsmIn i, bool softplus) {
   ssm_check(who, i, 2);
   if (!i.state.is_contiguous() || misaligned(i.state))
     refuse(text(who, ": state is updated in place and must be contiguous and 16-byte aligned"));
+  no_tracing(who);
   reverse_mode_only(who, {&i.x, &i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias});
   check_device(who, i.x, {&i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias});
   if (wants_grad({&i.x, &i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias}))

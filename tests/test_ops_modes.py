@@ -54,3 +54,12 @@ def test_forward_mode_tangents_are_refused_in_backward():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(y, a[0], dy, retain_graph=True)
         assert torch.isfinite(torch.autograd.grad(y, a[0], torch.ones_like(y))[0]).all()
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "causal_conv", "causal_conv_step", "ssm_scan", "ssm_step"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tracing_is_refused(name, grad):
+    """torch.jit.trace would record the result as a constant and the traced function would ignore its input."""
+    f, inputs = _inputs()[name]
+    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(f, tuple(inputs))
