@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kConvThreads, 2) k_conv_backward(const boa_con
     for (int i = 0; i < P; ++i) {
       const int k = i / V, j = i % V;
       const float v = joined[i * r.bx + gx];
-      if (k < K) out[(c + j) * K + k] = v;
+      if (k < K) out[(int64_t)(c + j) * K + k] = v;
       else out[(int64_t)K * E + c + j] = v;
     }
   }
@@ -403,9 +403,9 @@ static int conv_launch(const boa_conv_args& a, int what, cudaStream_t s) {
     if (smem > 48 * 1024)
       BOA_CUDA(cudaFuncSetAttribute(k_conv_backward<T, V, K>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     k_conv_backward<T, V, K><<<(unsigned)(blocks * r.group_blocks), kConvThreads, smem, s>>>(a, r, parts, blocks);
-    const int cols = (K + 1) * a.channels;
-    k_sum_parts<<<(cols + 31) / 32, 1024, 0, s>>>(parts, blocks, cols, K * a.channels, cols, a.dweight, a.dbias,
-                                                nullptr);
+    const int64_t cols = (K + 1LL) * a.channels;
+    k_sum_parts<<<(unsigned)((cols + 31) / 32), 1024, 0, s>>>(parts, blocks, cols, (int64_t)K * a.channels, cols,
+                                                             a.dweight, a.dbias, nullptr);
   }
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
@@ -436,6 +436,8 @@ static int conv_check(const boa_conv_args* a, const char* who) {
   if (!a) return boa_fail(BOA_ERR_ARG, std::string(who) + ": null arguments");
   if (a->batch < 0 || a->length < 0 || a->channels < 1)
     return boa_fail(BOA_ERR_ARG, std::string(who) + ": need batch >= 0, length >= 0 and channels >= 1");
+  if (a->length > kMaxSize || a->channels > kMaxSize)
+    return boa_fail(BOA_ERR_UNSUPPORTED, std::string(who) + ": length and channels must be below 2^31 - 2^16");
   if (a->width < 2 || a->width > 4) return boa_fail(BOA_ERR_UNSUPPORTED, std::string(who) + ": width must be 2, 3 or 4");
   if (a->dtype < BOA_DTYPE_F32 || a->dtype > BOA_DTYPE_F16)
     return boa_fail(BOA_ERR_ARG, std::string(who) + ": unknown dtype");

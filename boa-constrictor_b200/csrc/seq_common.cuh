@@ -343,12 +343,13 @@ __device__ __forceinline__ float warp_sum(float v) {
 // in a fixed order.  A block owns 32 columns; its 32 warps take the rows in turn
 // and are joined in shared memory.  Columns [0, s1) go to o1, [s1, s2) to o2 and
 // the rest to o3 (NULL: dropped), so one launch finishes up to three gradients.
-static __global__ void __launch_bounds__(1024) k_sum_parts(const float* __restrict__ parts, int64_t n_parts, int cols,
-                                                          int s1, int s2, float* __restrict__ o1,
-                                                          float* __restrict__ o2, float* __restrict__ o3) {
+static __global__ void __launch_bounds__(1024) k_sum_parts(const float* __restrict__ parts, int64_t n_parts,
+                                                          int64_t cols, int64_t s1, int64_t s2,
+                                                          float* __restrict__ o1, float* __restrict__ o2,
+                                                          float* __restrict__ o3) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (c < cols)
 #pragma unroll 8
@@ -364,6 +365,10 @@ static __global__ void __launch_bounds__(1024) k_sum_parts(const float* __restri
     else if (o3) o3[c - s2] = t;
   }
 }
+
+// Bound on the length and the channels of a call: indexes behind the last tile,
+// run or block of a row then still fit 32 bits.  Their products are 64 bits wide.
+constexpr int kMaxSize = 0x7fffffff - (1 << 16);
 
 inline bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 

@@ -882,10 +882,11 @@ __global__ void __launch_bounds__(256) k_ssm_bc(int64_t rows, int groups, const 
 // four elements.
 template <typename T, int ROWS, bool VEC>
 __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
-  const int E = a.channels, per = E * 4;
+  const int E = a.channels;
+  const int64_t per = E * 4LL;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t b0 = i / per * ROWS;
-  const int r = (int)(i % per), e = r >> 2, q = r & 3;
+  const int64_t b0 = i / per * ROWS, r = i % per;
+  const int e = (int)(r >> 2), q = (int)(r & 3);
   // the four lanes of a channel take the same streams: per and the block are multiples of four
   if (b0 >= a.batch) return;
   const unsigned mask = 0xfu << (threadIdx.x & 28);
@@ -953,7 +954,7 @@ static SsmPlan plan_forward(const boa_ssm_args& a) {
   }
   p.part = round_up((int)((a.length + parts - 1) / parts), kTile);
   if (p.part < kTile) p.part = kTile;
-  p.parts = a.length > 0 ? (a.length + p.part - 1) / p.part : 1;
+  p.parts = a.length > 0 ? (a.length - 1) / p.part + 1 : 1;
   return p;
 }
 
@@ -978,7 +979,7 @@ static SsmPlan plan_backward(const boa_ssm_args& a) {
     int64_t parts = 148LL * rounds / blocks;
     parts = parts < 1 ? 1 : parts < most ? parts : most < 1 ? 1 : most;
     const int part = round_up((int)((a.length + parts - 1) / parts), kBack);
-    const int n = part > 0 ? (a.length + part - 1) / part : 1;
+    const int n = part > 0 ? (a.length - 1) / part + 1 : 1;
     const int64_t cost = (blocks * n + 147) / 148 * (part + 6);
     if (best < 0 || cost * 100 <= best * 103) {
       p.part = part > kBack ? part : kBack;
@@ -1055,9 +1056,9 @@ static int ssm_backward_t(const boa_ssm_args& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.length, n = rows * 2 * kN;
   if (n > 0 && groups > 1)
     k_ssm_bc<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(rows, groups, bc, (T*)a.dB, (T*)a.dC);
-  const int cols = a.channels * (kN + 2);
-  k_sum_parts<<<(cols + 31) / 32, 1024, 0, s>>>(params, (int64_t)a.batch * p.parts, cols, a.channels * kN,
-                                              a.channels * (kN + 1), a.dA, a.dD, a.ddt_bias);
+  const int64_t E = a.channels, cols = E * (kN + 2);
+  k_sum_parts<<<(unsigned)((cols + 31) / 32), 1024, 0, s>>>(params, (int64_t)a.batch * p.parts, cols, E * kN,
+                                                           E * (kN + 1), a.dA, a.dD, a.ddt_bias);
   BOA_CUDA(cudaGetLastError());
   return BOA_OK;
 }
@@ -1069,7 +1070,7 @@ static int ssm_backward(const boa_ssm_args& a, cudaStream_t s) {
 
 template <typename T, int ROWS>
 static void ssm_step_rows(const boa_ssm_args& a, cudaStream_t s) {
-  const int64_t n = (a.batch + ROWS - 1LL) / ROWS * a.channels * 4;
+  const int64_t n = (a.batch + (ROWS - 1LL)) / ROWS * a.channels * 4;
   const unsigned grid = (unsigned)((n + 255) / 256);
   if (row_vec(a.B, a.B_bs, 0, sizeof(T)) && row_vec(a.C, a.C_bs, 0, sizeof(T)))
     k_ssm_step<T, ROWS, true><<<grid, 256, 0, s>>>(a);
@@ -1090,6 +1091,8 @@ static int ssm_check(const boa_ssm_args* a, const char* who) {
   if (!a) return boa_fail(BOA_ERR_ARG, std::string(who) + ": null arguments");
   if (a->batch < 0 || a->length < 0 || a->channels < 1)
     return boa_fail(BOA_ERR_ARG, std::string(who) + ": need batch >= 0, length >= 0 and channels >= 1");
+  if (a->length > kMaxSize || a->channels > kMaxSize)
+    return boa_fail(BOA_ERR_UNSUPPORTED, std::string(who) + ": length and channels must be below 2^31 - 2^16");
   if (a->states != kN) return boa_fail(BOA_ERR_UNSUPPORTED, std::string(who) + ": states must be 16");
   if (a->dtype < BOA_DTYPE_F32 || a->dtype > BOA_DTYPE_F16)
     return boa_fail(BOA_ERR_ARG, std::string(who) + ": unknown dtype");

@@ -254,11 +254,12 @@ BOA_API int boa_codec_decode_range(boa_model* m, int n_chunks, const uint32_t* d
 /* statistics, scan states and parameter gradients are fp32.  Sequences are  */
 /* [batch, length, channels] with channels contiguous; *_bs and *_ts are the */
 /* batch and token strides in elements, so slices of wider rows need no      */
-/* copy.  Outputs are contiguous.  Every call only enqueues work on `stream` */
-/* and runs on device `device`; nothing is kept between calls.  Sums have a  */
-/* fixed order: equal inputs give equal bits on equal devices, but a row's   */
-/* last bits may depend on the sizes of the call (the scan's split of the    */
-/* length follows them).                                                     */
+/* copy.  Outputs are contiguous.  length and channels of the convolution    */
+/* and the scan are below 2^31 - 2^16 (BOA_ERR_UNSUPPORTED).  Every call     */
+/* only enqueues work on `stream` and runs on device `device`; nothing is    */
+/* kept between calls.  Sums have a fixed order: equal inputs give equal     */
+/* bits on equal devices, but a row's last bits may depend on the sizes of   */
+/* the call (the scan's split of the length follows them).                   */
 /* ------------------------------------------------------------------------ */
 #define BOA_DTYPE_F32 0
 #define BOA_DTYPE_BF16 1
