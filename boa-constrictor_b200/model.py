@@ -298,15 +298,24 @@ class BoaBytePredictor(nn.Module):
         if not self.embedding.weight.is_cuda:
             raise RuntimeError(f"{who} runs on CUDA devices only (no CPU path): move the model with .cuda()")
 
+    def _embed(self, x, lens=None):
+        """Embedded tokens; what a row holds behind its valid length is no token (padding of any value)."""
+        x = x.to(self.embedding.weight.device).long()
+        if lens is not None:
+            if lens.shape != x.shape[:1]:
+                raise ValueError(f"lens must have shape {tuple(x.shape[:1])}, got {tuple(lens.shape)}")
+            x = x.masked_fill(torch.arange(x.shape[1], device=x.device) >= lens[:, None], 0)
+        return self.embedding(x)
+
     def forward_layers(self, x, state=None, lens=None, return_state: bool = False):
         """x [B, L] -> logits [B, L, vocab], differentiable in every parameter.
 
-        ``lens`` [B] gives the valid length of each row (the logits behind it
-        are computed from zeros and mean nothing).  ``state`` continues a
+        ``lens`` [B] gives the valid length of each row (what x holds behind it
+        is not read, the logits there mean nothing).  ``state`` continues a
         sequence; with ``return_state`` the result is (logits, state behind
         every row's last valid position) for a later call or ``step_layers``."""
         self._check_tokens("forward_layers", x, 2)
-        h = self.embedding(x.to(self.embedding.weight.device).long())
+        h = self._embed(x, lens)
         out = []
         for i, block in enumerate(self.blocks):
             h, s = block(h, None if state is None else state[i], lens, return_state=True)
