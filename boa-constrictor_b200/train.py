@@ -38,7 +38,11 @@ def train_step(model, batch, optimizer, criterion, lens=None) -> torch.Tensor:
     """One step on a batch of byte rows [B, L]: predict bytes 1..L-1 from
     0..L-2, ``criterion(logits, targets)``, backward, ``optimizer.step()``.
     ``lens`` [B] is the number of valid bytes of each row; what lies behind
-    takes no part.  Returns the loss (on the device, nothing is synchronised)."""
+    takes no part.  Returns the loss (on the device, nothing is synchronised).
+
+    Called within ``torch.autocast``, the forward part and the loss run in it,
+    the backward pass and the optimizer outside of it; the casts of the weights
+    that autocast keeps for its region are dropped, since the step changes them."""
     dev = model.embedding.weight.device
     batch = batch.to(dev)
     inputs, targets = batch[:, :-1], batch[:, 1:].long()
@@ -49,8 +53,10 @@ def train_step(model, batch, optimizer, criterion, lens=None) -> torch.Tensor:
     optimizer.zero_grad(set_to_none=True)
     logits = model.forward_layers(inputs, lens=lens)
     loss = criterion(logits.reshape(-1, logits.shape[-1]), targets.reshape(-1))
-    loss.backward()
-    optimizer.step()
+    with torch.autocast(dev.type, enabled=False):
+        loss.backward()
+        optimizer.step()
+    torch.clear_autocast_cache()
     return loss.detach()
 
 

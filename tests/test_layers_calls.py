@@ -50,3 +50,70 @@ def test_padding_takes_no_part():
     # the embedding's gradient is summed by torch in no fixed order: some rounding of its largest values
     for a, b in zip(*out):
         assert torch.isfinite(a).all() and (a - b).norm() <= 1e-6 * b.norm()
+
+
+# ------------------------------------------------------------------- autocast
+class _Small(torch.nn.Module):
+    """A predictor with forward_layers that runs anywhere."""
+
+    def __init__(self):
+        super().__init__()
+        self.embedding = torch.nn.Embedding(256, 16)
+        self.head = torch.nn.Linear(16, 256)
+
+    def forward_layers(self, x, lens=None):
+        return self.head(self.embedding(x.long()))
+
+
+def _steps(m, batches, dev, around_all):
+    """One optimizer step a batch in bf16: all in one autocast region, or each in its own."""
+    from train import train_step
+    opt = torch.optim.SGD(m.parameters(), lr=0.5)
+    losses = []
+    if around_all:
+        with torch.autocast(dev, torch.bfloat16):
+            for b in batches:
+                losses.append(train_step(m, b, opt, F.cross_entropy))
+            last = m.forward_layers(batches[0].to(dev))         # sees the weights of the last step
+    else:
+        for b in batches:
+            with torch.autocast(dev, torch.bfloat16):
+                losses.append(train_step(m, b, opt, F.cross_entropy))
+        with torch.autocast(dev, torch.bfloat16):
+            last = m.forward_layers(batches[0].to(dev))
+    return losses, last.detach(), {k: v.detach().clone() for k, v in m.state_dict().items()}
+
+
+def _same_steps(make, dev, tolerance):
+    batches = [_bytes(4, 12, 20 + i) for i in range(3)]
+    one, two = (_steps(make(), batches, dev, around) for around in (True, False))
+    for a, b in zip(one[0] + [one[1]] + list(one[2].values()), two[0] + [two[1]] + list(two[2].values())):
+        assert (a - b).float().norm() <= tolerance * b.float().norm()
+
+
+def test_steps_in_one_autocast_region_use_their_own_weights():
+    """Autocast keeps the bf16 copies of weights for as long as the region lasts; a step changes the weights."""
+    def make():
+        torch.manual_seed(0)
+        return _Small()
+    _same_steps(make, "cpu", 0.0)
+
+
+@pytest.mark.gpu
+def test_steps_in_one_autocast_region_use_their_own_weights_gpu():
+    """With forward_layers.  The embedding's gradient is summed by torch in no fixed order; a weight that moves by one
+    fp32 rounding can move its bf16 copy by one step of 2^-8, few of them do."""
+    _same_steps(lambda: _model(64, 1).cuda(), "cuda", 1e-3)
+
+
+def test_backward_and_optimizer_run_outside_autocast():
+    m = _Small()
+    seen = []
+    m.head.weight.register_hook(lambda g: seen.append(torch.is_autocast_enabled("cpu")))
+    opt = torch.optim.SGD(m.parameters(), lr=0.1)
+    opt.register_step_pre_hook(lambda *a: seen.append(torch.is_autocast_enabled("cpu")))
+    from train import train_step
+    with torch.autocast("cpu", torch.bfloat16):
+        train_step(m, _bytes(2, 5, 3), opt, F.cross_entropy)
+        assert torch.is_autocast_enabled("cpu")
+    assert seen == [False, False]
