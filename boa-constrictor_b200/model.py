@@ -213,6 +213,7 @@ class NativeModel:
 
 class BoaBytePredictor(nn.Module):
     """Mamba model predicting the next byte (model.py:83-131)."""
+    _captured = False       # whether a CUDA graph may hold a training step of these parameters
 
     def __init__(self, d_model=256, num_layers=4, vocab_size=256, weight_format: str | None = None):
         super().__init__()
@@ -231,6 +232,13 @@ class BoaBytePredictor(nn.Module):
     def _param_key(self):
         return tuple((id(p), p._version) for p in self.parameters()), self.weight_format
 
+    def _param_values(self):
+        """All parameters in one tensor: what a replayed graph changes without moving a version."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured training step may have changed the parameters, and they cannot be read "
+                               "while another capture runs: capture the fused kernel with a model of its own")
+        return torch.cat([p.detach().reshape(-1).float() for p in self.parameters()])
+
     def _native_handle(self, device) -> NativeModel:
         device = torch.device(device)
         if device.type != "cuda":
@@ -239,10 +247,11 @@ class BoaBytePredictor(nn.Module):
         idx = device.index if device.index is not None else torch.cuda.current_device()
         key = (idx,) + self._param_key()
         nm = self._native.get(idx)
-        if nm is None or nm[0] != key:
+        values = self._param_values() if self._captured else None
+        if nm is None or nm[0] != key or (values is not None and (nm[2] is None or not torch.equal(nm[2], values))):
             sd = {k: v.detach().float().cpu() for k, v in self.state_dict().items()}
             self._native[idx] = (key, NativeModel(sd, self.d_model, self.num_layers, self.vocab_size,
-                                                  WEIGHT_FORMATS[self.weight_format], idx))
+                                                  WEIGHT_FORMATS[self.weight_format], idx), values)
         return self._native[idx][1]
 
     def native(self, device=None) -> NativeModel:
@@ -315,6 +324,7 @@ class BoaBytePredictor(nn.Module):
         sequence; with ``return_state`` the result is (logits, state behind
         every row's last valid position) for a later call or ``step_layers``."""
         self._check_tokens("forward_layers", x, 2)
+        self._captured |= torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()
         h = self._embed(x, lens)
         out = []
         for i, block in enumerate(self.blocks):

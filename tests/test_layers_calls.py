@@ -117,3 +117,46 @@ def test_backward_and_optimizer_run_outside_autocast():
         train_step(m, _bytes(2, 5, 3), opt, F.cross_entropy)
         assert torch.is_autocast_enabled("cpu")
     assert seen == [False, False]
+
+
+# ------------------------------------------------------------------- captured steps
+def _capture_step(m, batch):
+    """A graph of one optimizer step, behind the steps on another stream that such a capture wants."""
+    from train import train_step
+    opt = torch.optim.SGD(m.parameters(), lr=0.5)
+    step = lambda: train_step(m, batch, opt, F.cross_entropy)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    return graph, loss
+
+
+@pytest.mark.gpu
+def test_fused_kernel_takes_the_weights_of_replayed_steps():
+    """A replay changes the parameters without moving their versions; the fused kernel's copy of them follows."""
+    m = _model(64, 1).cuda()
+    batch = _bytes(4, 17, 30).cuda()
+    graph, loss = _capture_step(m, batch)
+
+    def agree():
+        with torch.no_grad():
+            p = torch.softmax(m.forward_layers(batch), -1)
+        assert (p - torch.softmax(m(batch), -1)).abs().max() < 1e-4
+        return p
+
+    before, losses = agree(), []
+    for _ in range(3):
+        graph.replay()
+        losses.append(loss.clone())
+        after = agree()
+        assert (after - before).abs().max() > 1e-3          # the step did change the model
+        before = after
+    assert torch.isfinite(torch.stack(losses)).all()
+    handle = m.native()
+    assert m.native() is handle                             # and is made once for the same weights
