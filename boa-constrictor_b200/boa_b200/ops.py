@@ -102,3 +102,10 @@ def ssm_step(x, dt, state, A, B, C, D=None, z=None, dt_bias=None, *, softplus: b
     ``B, C [batch, 16]`` -> ``y [batch, channels]``; ``state [batch, channels, 16]``
     (float32, contiguous, 16-byte aligned) is updated in place."""
     return _boa_ops.ssm_step(x, dt, state, A, B, C, D, z, dt_bias, softplus)
+
+
+def held_on_default_stream(parameters) -> bool:
+    """Whether an autograd graph that is still alive would add to the gradient of
+    one of ``parameters`` on the default stream: a backward pass must not be
+    captured then."""
+    return _boa_ops.held_on_default_stream(tuple(parameters))

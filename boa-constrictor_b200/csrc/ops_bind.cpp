@@ -662,6 +662,25 @@ PyObject* py_ssm_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
                     flag(a[9]));
   });
 }
+// held_on_default_stream(parameters): whether an autograd graph that is still alive would accumulate into one of them on
+// its device's default stream, which cannot take part in a capture.
+PyObject* py_held(PyObject*, PyObject* list) {
+  HANDLE_TH_ERRORS
+  PyObject* seq = PySequence_Fast(list, "a sequence of tensors");
+  if (!seq) return nullptr;
+  bool held = false;
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq) && !held; ++i) {
+    PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
+    if (!THPVariable_Check(o) || !THPVariable_Unpack(o).is_cuda()) continue;
+    const Tensor& t = THPVariable_Unpack(o);
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    held = stream && *stream == c10::cuda::getDefaultCUDAStream(t.get_device()).unwrap();
+  }
+  Py_DECREF(seq);
+  return PyBool_FromLong(held);
+  END_HANDLE_TH_ERRORS
+}
 // bind(loader, BoaError)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) {
@@ -688,6 +707,7 @@ PyMethodDef methods[] = {
     {"causal_conv_step", fast(py_causal_conv_step), METH_FASTCALL, "x, state, weight, bias, silu"},
     {"ssm_scan", fast(py_ssm_scan), METH_FASTCALL, "x, dt, A, B, C, D, z, dt_bias, softplus, state, lens, return_state"},
     {"ssm_step", fast(py_ssm_step), METH_FASTCALL, "x, dt, state, A, B, C, D, z, dt_bias, softplus"},
+    {"held_on_default_stream", py_held, METH_O, "parameters"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_boa_ops", "host side of boa_b200.ops", -1, methods};
 

@@ -16,6 +16,8 @@ import math
 
 import torch
 
+from boa_b200 import ops
+
 
 @torch.inference_mode()
 def evaluate_bpp(model, loader, criterion, device="cuda", vocab_size=256) -> float:
@@ -42,8 +44,16 @@ def train_step(model, batch, optimizer, criterion, lens=None) -> torch.Tensor:
 
     Called within ``torch.autocast``, the forward part and the loss run in it,
     the backward pass and the optimizer outside of it; the casts of the weights
-    that autocast keeps for its region are dropped, since the step changes them."""
+    that autocast keeps for its region are dropped, since the step changes them.
+
+    It can be captured into a CUDA graph, behind a few steps on another stream.
+    Autograd adds to a parameter's gradient on the stream of the oldest graph
+    that is alive; on the default stream the capture would end the process, so
+    it is refused while an output of an earlier call keeps such a graph."""
     dev = model.embedding.weight.device
+    if dev.type == "cuda" and torch.cuda.is_current_stream_capturing() and ops.held_on_default_stream(model.parameters()):
+        raise RuntimeError("train_step cannot be captured while a loss or an output of an earlier call keeps its autograd "
+                           "graph alive: delete it first")
     batch = batch.to(dev)
     inputs, targets = batch[:, :-1], batch[:, 1:].long()
     if lens is not None:

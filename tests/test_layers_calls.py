@@ -160,3 +160,29 @@ def test_fused_kernel_takes_the_weights_of_replayed_steps():
     assert torch.isfinite(torch.stack(losses)).all()
     handle = m.native()
     assert m.native() is handle                             # and is made once for the same weights
+
+
+@pytest.mark.gpu
+def test_a_step_is_not_captured_over_a_living_graph():
+    """An output of an earlier call keeps its graph, whose gradients are added on the default stream: refused before
+    anything is captured.  Without it the step is captured."""
+    from boa_b200 import ops
+    from train import train_step
+    m = _model(64, 1).cuda()
+    batch = _bytes(2, 9, 31).cuda()
+    opt = torch.optim.SGD(m.parameters(), lr=0.5)
+    assert not ops.held_on_default_stream(m.parameters())
+    kept = m.forward_layers(batch)
+    assert ops.held_on_default_stream(m.parameters())
+    before = [p.detach().clone() for p in m.parameters()]
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            train_step(m, batch, opt, F.cross_entropy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, b) for p, b in zip(m.parameters(), before))
+    train_step(m, batch, opt, F.cross_entropy)              # outside of a capture nothing is refused
+    del kept
+    assert not ops.held_on_default_stream(m.parameters())
+    graph, loss = _capture_step(m, batch)
+    graph.replay()
+    assert torch.isfinite(loss)
