@@ -265,7 +265,9 @@ static void norm_launch(const NormCall& c, bool backward) {
   if (backward) {
     const size_t smem = (size_t)2 * c.width * sizeof(float);
     auto k = k_norm_backward<T, V, VPL, ROW_WARPS>;
-    if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // the bound of all widths, not this one's size: another thread may launch between here and the launch
+    if (smem > 48 * 1024)
+      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kNormMaxWidth * (int)sizeof(float));
     k<<<c.grid, kNormWarps * 32, smem, c.s>>>(c.rows, c.width, (const T*)c.x, c.x_stride, (const T*)c.dy, c.dy_stride,
                                              c.w, c.stats, (T*)c.out, c.parts);
   } else {

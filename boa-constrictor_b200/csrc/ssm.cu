@@ -1050,7 +1050,9 @@ static int ssm_backward_t(const boa_ssm_args& a, cudaStream_t s) {
   BOA_CUDA(cudaFuncGetAttributes(&fa, k_ssm_backward<T, VEC>));
   if (fa.numRegs != kBackRegs)
     return boa_fail(BOA_ERR_UNSUPPORTED, "boa_ssm_scan_backward: built with another register count than its split");
-  BOA_CUDA(cudaFuncSetAttribute(k_ssm_backward<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the bound of all calls, not this one's size: another thread may launch between here and the launch
+  BOA_CUDA(cudaFuncSetAttribute(k_ssm_backward<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                BackSmem::floats(kPasses) * (int)sizeof(float)));
   k_ssm_backward<T, VEC><<<(unsigned)((int64_t)groups * p.parts * a.batch), kBackThreads, smem, s>>>(a, p, passes, groups,
                                                                                              ends, bc, params);
   const int64_t rows = (int64_t)a.batch * a.length, n = rows * 2 * kN;
