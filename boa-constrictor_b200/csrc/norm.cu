@@ -328,6 +328,7 @@ BOA_API int boa_layer_norm(int64_t rows, int width, int dtype, const void* d_x, 
   if (rc) return rc;
   if (rows == 0) return BOA_OK;
   if (!d_x || !d_weight || !d_y) return boa_fail(BOA_ERR_ARG, "boa_layer_norm: null argument");
+  if (!aligned(d_stats, 8)) return boa_fail(BOA_ERR_ARG, "boa_layer_norm: stats must be 8-byte aligned");
   BOA_CUDA(cudaSetDevice(device));
   NormCall c{};
   c.rows = rows; c.width = width; c.dtype = dtype; c.x = d_x; c.x_stride = x_stride;
@@ -359,6 +360,7 @@ BOA_API int boa_layer_norm_backward(int64_t rows, int width, int dtype, const vo
   }
   if (!d_x || !d_dy || !d_weight || !d_stats || !d_dx)
     return boa_fail(BOA_ERR_ARG, "boa_layer_norm_backward: null argument");
+  if (!aligned(d_stats, 8)) return boa_fail(BOA_ERR_ARG, "boa_layer_norm_backward: stats must be 8-byte aligned");
   if (!d_workspace || workspace_bytes < boa_layer_norm_workspace_bytes(rows, width, dtype))
     return boa_fail(BOA_ERR_ARG, "boa_layer_norm_backward: workspace too small (see boa_layer_norm_workspace_bytes)");
   BOA_CUDA(cudaSetDevice(device));

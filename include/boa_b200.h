@@ -267,9 +267,9 @@ BOA_API int boa_codec_decode_range(boa_model* m, int n_chunks, const uint32_t* d
 
 /* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis
  * (nn.LayerNorm, model.py:45,51).  x is [rows, width] with row stride x_stride;
- * y is contiguous; bias may be NULL.  stats (NULL, or 2 * rows floats) receives
- * mean and 1/sqrt(var + eps) of every row for the backward call.  width is in
- * [1, 8192] (BOA_ERR_UNSUPPORTED beyond). */
+ * y is contiguous; bias may be NULL.  stats (NULL, or 2 * rows floats, 8-byte
+ * aligned) receives mean and 1/sqrt(var + eps) of every row for the backward
+ * call.  width is in [1, 8192] (BOA_ERR_UNSUPPORTED beyond). */
 BOA_API int boa_layer_norm(int64_t rows, int width, int dtype, const void* d_x, int64_t x_stride,
                            const float* d_weight, const float* d_bias, float eps, void* d_y, float* d_stats,
                            int device, void* stream);
