@@ -307,6 +307,10 @@ class BoaBytePredictor(nn.Module):
         if not self.embedding.weight.is_cuda:
             raise RuntimeError(f"{who} runs on CUDA devices only (no CPU path): move the model with .cuda()")
 
+    def _check_state(self, who, state):
+        if len(state) != len(self.blocks):
+            raise ValueError(f"{who}: the model has {len(self.blocks)} blocks, the state holds {len(state)}")
+
     def _embed(self, x, lens=None):
         """Embedded tokens; what a row holds behind its valid length is no token (padding of any value)."""
         x = x.to(self.embedding.weight.device).long()
@@ -324,6 +328,8 @@ class BoaBytePredictor(nn.Module):
         sequence; with ``return_state`` the result is (logits, state behind
         every row's last valid position) for a later call or ``step_layers``."""
         self._check_tokens("forward_layers", x, 2)
+        if state is not None:
+            self._check_state("forward_layers", state)
         self._captured |= torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing()
         h = self._embed(x, lens)
         out = []
@@ -341,6 +347,7 @@ class BoaBytePredictor(nn.Module):
     def step_layers(self, byte_t, state):
         """byte_t [B] -> logits [B, vocab]; ``state`` moves on in place."""
         self._check_tokens("step_layers", byte_t, 1)
+        self._check_state("step_layers", state)
         h = self.embedding(byte_t.to(self.embedding.weight.device).long())
         for block, s in zip(self.blocks, state):
             h = block.step(h, s)

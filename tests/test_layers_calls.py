@@ -186,3 +186,30 @@ def test_a_step_is_not_captured_over_a_living_graph():
     graph, loss = _capture_step(m, batch)
     graph.replay()
     assert torch.isfinite(loss)
+
+
+# ------------------------------------------------------------------- states of another model
+def test_states_of_another_depth_are_refused():
+    """One state a block: fewer left the last blocks out of a step, more were ignored."""
+    m = _model(64, 2)
+    one = m.init_layers(3)
+    for bad in (one[:1], one + one[:1], []):
+        with pytest.raises(ValueError, match="2 blocks"):
+            m._check_state("step_layers", bad)
+    m._check_state("step_layers", one)
+
+
+@pytest.mark.gpu
+def test_states_of_another_depth_are_refused_gpu():
+    m = _model(64, 2).cuda()
+    x = _bytes(3, 4, 40).cuda()
+    state = m.init_layers(3)
+    for bad in (state[:1], state + state[:1]):
+        with pytest.raises(ValueError, match="2 blocks"):
+            m.step_layers(x[:, 0], bad)
+        with pytest.raises(ValueError, match="2 blocks"):
+            m.forward_layers(x, bad)
+    assert all(not t.any() for s in state for t in s)
+    with torch.no_grad():
+        m.forward_layers(x, state)
+        m.step_layers(x[:, 0], state)
