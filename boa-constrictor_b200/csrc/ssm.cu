@@ -97,6 +97,13 @@ __device__ __forceinline__ void load_pairs(const float* p, int c, int E, f2 (&v)
   v[0] = pack(t[0], t[1]);
   v[1] = pack(t[2], t[3]);
 }
+// A in units of log2, for a decay ex2(d rate).  -inf (a channel that forgets at
+// once) is held at the lowest number: d is 0 behind a row's end, where the decay
+// is 1 and 0 times -inf would not be.
+__device__ __forceinline__ float rate_of(float A) {
+  const float r = A * kLog2e;
+  return r < -3.402823466e38f ? -3.402823466e38f : r;
+}
 __device__ __forceinline__ float step_of(float raw, bool softplus) {
   float u;
   return softplus ? softplus_f(raw, u) : raw;
@@ -159,7 +166,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) k_ssm(const boa_ssm_args a, c
                         : a.state   ? a.state + ((int64_t)b * E + e) * kN : nullptr;
 #pragma unroll
       for (int j = 0; j < kQ; ++j) {
-        v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+        v[j] = on ? rate_of(a.A[(int64_t)e * kN + kQ * q + j]) : 0.0f;
         s[j] = on && s0 ? s0[kQ * q + j] : 0.0f;
       }
       A2[0] = pack(v[0], v[1]);
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_ends(const boa_ssm_args a, 
   {
     float v[kQ];
 #pragma unroll
-    for (int j = 0; j < kQ; ++j) v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+    for (int j = 0; j < kQ; ++j) v[j] = on ? rate_of(a.A[(int64_t)e * kN + kQ * q + j]) : 0.0f;
     A2[0] = pack(v[0], v[1]);
     A2[1] = pack(v[2], v[3]);
   }
@@ -367,7 +374,7 @@ static __global__ void __launch_bounds__(128) k_ssm_join(int64_t n, int E, int p
   if (i >= n) return;
   const int64_t en = (int64_t)E * kN;
   const int64_t b = i / en, r = i % en;
-  const float A2 = A[r] * kLog2e;
+  const float A2 = rate_of(A[r]);
   float carry = first ? first[i] : 0.0f;
   const int64_t step = reverse ? -1 : 1;
   int64_t s = b * parts + (reverse ? parts - 1 : 0);
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(kSsmThreads) k_ssm_back_ends(const boa_ssm_arg
   {
     float v[kQ];
 #pragma unroll
-    for (int j = 0; j < kQ; ++j) v[j] = on ? a.A[(int64_t)e * kN + kQ * q + j] * kLog2e : 0.0f;
+    for (int j = 0; j < kQ; ++j) v[j] = on ? rate_of(a.A[(int64_t)e * kN + kQ * q + j]) : 0.0f;
     A2[0] = pack(v[0], v[1]);
     A2[1] = pack(v[2], v[3]);
   }
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
           v = make_float4(s[0], s[1], s[2], s[3]);
         }
         const float* s = a.A + (int64_t)e * kN + kQ * q;
-        A = make_float4(s[0] * kLog2e, s[1] * kLog2e, s[2] * kLog2e, s[3] * kLog2e);
+        A = make_float4(rate_of(s[0]), rate_of(s[1]), rate_of(s[2]), rate_of(s[3]));
       }
       st4(dh_s + at, v);
       st4(dA_s + at, make_float4(0.f, 0.f, 0.f, 0.f));
@@ -650,6 +657,7 @@ __global__ void __launch_bounds__(kBackThreads, 1)
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < kBackScan / 32; ++w) s += sm[S::red + w * S::kBc + tid];
+        if (t >= end) s = 0.0f;
         const int64_t rowi = (int64_t)b * a.length + t;
         if (t < stop) {
           if (groups > 1) bc_parts[((int64_t)group * a.batch * a.length + rowi) * 2 * kN + n] = s;
@@ -756,9 +764,10 @@ __global__ void __launch_bounds__(kBackThreads, 1)
       ld2(db, ab);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        ox[j] = fma2(s1[j], pd2[j], mul2(Dv[j], pg2[j]));
+        // behind the row's end every gradient is 0, whatever D or the gradient of the state hold
+        ox[j] = in_row ? fma2(s1[j], pd2[j], mul2(Dv[j], pg2[j])) : f2{0ull};
         od[j] = in_row ? mul2(fma2(s1[j], px2[j], mul2(ln2, s2[j])), ps[j]) : f2{0ull};   // s2 is in units of log2
-        oz[j] = gated ? mul2(pz2[j], fma2(Dv[j], px2[j], sv[j])) : f2{0ull};
+        oz[j] = gated && in_row ? mul2(pz2[j], fma2(Dv[j], px2[j], sv[j])) : f2{0ull};
         aD[j] = fma2(pg2[j], px2[j], aD[j]);
         ab[j] = add2(ab[j], od[j]);
       }
@@ -907,7 +916,7 @@ __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
       if (a.z) z[k] = ((const T*)a.z)[b * a.z_bs + e];
     }
   const float4 A4 = *reinterpret_cast<const float4*>(a.A + (int64_t)e * kN + kQ * q);
-  const f2 A2[2] = {pack(A4.x * kLog2e, A4.y * kLog2e), pack(A4.z * kLog2e, A4.w * kLog2e)};
+  const f2 A2[2] = {pack(rate_of(A4.x), rate_of(A4.y)), pack(rate_of(A4.z), rate_of(A4.w))};
   const float bias = a.dt_bias ? a.dt_bias[e] : 0.0f, D = a.D ? a.D[e] : 0.0f;
 #pragma unroll
   for (int k = 0; k < ROWS; ++k) {

@@ -63,3 +63,51 @@ def test_tracing_is_refused(name, grad):
     f, inputs = _inputs()[name]
     with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(f, tuple(inputs))
+
+
+# ------------------------------------------------------------------- values that are not finite, behind a row's end
+@pytest.mark.gpu
+@pytest.mark.parametrize("E", [24, 33])
+def test_scan_gradients_behind_a_row_are_zero_whatever_the_rest_holds(E):
+    """D, the gradient of the final state or A of inf or NaN reach the tokens of a row, not those behind its end."""
+    g = torch.Generator().manual_seed(E)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    lens = torch.tensor([0, 3, 11, 16, 17], device="cuda")
+    leaves = [r(5, 18, E), r(5, 18, E), r(5, 18, 16), r(5, 18, 16), r(5, 18, E)]
+    A, D, dout = -torch.rand(E, 16, generator=g).cuda(), r(E), r(5, E, 16)
+    A[3], D[::2], dout[:, 5] = float("nan"), float("inf"), float("inf")
+    x, dt, B, C, z = (t.requires_grad_() for t in leaves)
+    y, out = ops.ssm_scan(x, dt, A, B, C, D, z, lens=lens, return_state=True)
+    grads = torch.autograd.grad((y, out), (x, dt, B, C, z), (r(5, 18, E), dout))
+    behind = torch.arange(18, device="cuda") >= lens[:, None]
+    for name, t in zip(("y", "dx", "ddt", "dB", "dC", "dz"), (y,) + grads):
+        assert (t[behind] == 0).all(), name
+
+
+@pytest.mark.gpu
+def test_scan_channels_that_forget_at_once():
+    """A of -inf: the decay is 0 at every token and 1 behind a row's end, forward, backward and for single tokens."""
+    import ops_reference as ref
+    g = torch.Generator().manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    nb, length, e = 3, 21, 24
+    x, dt, z, dy = (r(nb, length, e) for _ in range(4))
+    B, C = r(nb, length, 16), r(nb, length, 16)
+    A, D, bias, state, dout = -torch.rand(e, 16, generator=g), r(e), r(e), r(nb, e, 16), r(nb, e, 16)
+    A[::3], A[1, 4] = float("-inf"), float("-inf")
+    lens = torch.tensor([21, 1, 13], dtype=torch.int32)
+    # in the reference a decay that is 0 from the smallest d on, but with a product of 0 behind the row
+    far = torch.where(A == float("-inf"), torch.tensor(-1e30), A)
+    want = ref.scan(*[t.double() for t in (x, dt, far, B, C, D, z, bias)], True, state.double(), lens, dy.double(),
+                    dout.double())
+    names = ("dx", "ddt", "dA", "dB", "dC", "dD", "dz", "dbias", "dstate")
+    leaves = [t.cuda().requires_grad_() for t in (x, dt, A, B, C, D, z, bias, state)]
+    y, out = ops.ssm_scan(*leaves[:8], state=leaves[8], lens=lens.cuda(), return_state=True)
+    grads = torch.autograd.grad((y, out), leaves, (dy.cuda(), dout.cuda()))
+    # counts of the scan's own tests: 8 a token and 64, twice and more where two such results meet or rows are summed
+    for name, t in zip(("y", "state") + names, (y, out) + grads):
+        ref.close(name, t, *want[name], 16 * length + 128 + nb * length / 8)
+    st = state.cuda()
+    with torch.no_grad():
+        one = ops.ssm_step(x[:, 0].cuda(), torch.full((nb, e), -200.0).cuda(), st, A.cuda(), B[:, 0].cuda(), C[:, 0].cuda())
+    assert torch.equal(st, state.cuda()) and torch.isfinite(one).all()      # d underflows to 0: nothing moves
