@@ -162,6 +162,16 @@ Tensor param(const Tensor& t) {
 Tensor rows(const Tensor& t) {
   return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
+// An input of a step apart from the state that the step changes in place: one that shares its memory would be read by
+// some threads after others have written it.
+Tensor apart(const Tensor& t, const Tensor& state) {
+  if (!t.defined() || t.numel() == 0 || state.numel() == 0) return t;
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const char *begin = static_cast<const char*>(t.data_ptr()), *end = begin + (last + 1) * (int64_t)t.element_size();
+  const char *from = static_cast<const char*>(state.data_ptr()), *to = from + state.nbytes();
+  return begin < to && from < end ? t.clone(at::MemoryFormat::Contiguous) : t;
+}
 Tensor int_lens(const char* who, const Tensor& lens, int64_t batch, int64_t length) {
   if (!lens.defined()) return lens;
   if (lens.scalar_type() != at::kInt && lens.scalar_type() != at::kLong)
@@ -392,8 +402,8 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   if (wants_grad({&x_, &state, &w, &bias}))
     throw Refused{PyExc_RuntimeError,
                   text(who, " has no gradient: call it under torch.no_grad(), or use causal_conv")};
-  w = param(w);
-  const Tensor b = param(bias), x = rows(x_);
+  w = apart(param(w), state);
+  const Tensor b = apart(param(bias), state), x = apart(rows(x_), state);
   OnDevice on(x);
   Tensor y = like(x);
   boa_conv_args a = conv_args(x, w, b, silu, Tensor(), Tensor());
@@ -571,6 +581,7 @@ Tensor ssm_step(SsmIn i, bool softplus) {
   if (wants_grad({&i.x, &i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias}))
     throw Refused{PyExc_RuntimeError, text(who, " has no gradient: call it under torch.no_grad(), or use ssm_scan")};
   ssm_prepare(i);
+  for (Tensor* t : {&i.x, &i.dt, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias}) *t = apart(*t, i.state);
   OnDevice on(i.x);
   Tensor y = like(i.x);
   boa_ssm_args a = ssm_args(i, softplus);
