@@ -30,6 +30,7 @@ There is no CPU path: tensors that are not on a CUDA device raise RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import importlib
 
 import torch  # noqa: F401  (before _boa_ops, which links to it)
 
@@ -44,19 +45,22 @@ def _addresses():
     return {n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ["boa_last_error"] + _ENTRY_POINTS}
 
 
-try:
-    from . import _boa_ops
-except ImportError as e:                                    # not built
-    class _Missing:
-        """Raises on every call, like a missing libboa_b200.so."""
-        reason = str(e)
+class _OnFirstUse:
+    """Stands for _boa_ops until its first call, so that a program that runs only
+    the codec does not load it; raises if it was not built."""
 
-        def __getattr__(self, name):
-            raise RuntimeError(f"_boa_ops is not built ({self.reason}); run __graft_entry__.build()")
+    def __getattr__(self, name):
+        global _boa_ops
+        try:
+            module = importlib.import_module("._boa_ops", __package__)
+        except ImportError as e:
+            raise RuntimeError(f"_boa_ops is not built ({e}); run __graft_entry__.build()") from e
+        module.bind(_addresses, _n.BoaError)
+        _boa_ops = module
+        return getattr(module, name)
 
-    _boa_ops = _Missing()
-else:
-    _boa_ops.bind(_addresses, _n.BoaError)
+
+_boa_ops = _OnFirstUse()
 
 
 def layer_norm(x, weight, bias=None, eps: float = 1e-5):
