@@ -47,3 +47,13 @@ for _ in range(2):
         print('not built' in str(e))
 """).split()
     assert out == ["True", "True"]
+
+
+def test_the_library_is_built_without_torch_headers(tmp_path):
+    """`make lib` is every step of libboa_b200.so and none that wants torch or g++."""
+    make = ["make", "-n", "-C", os.path.join(PKG, "csrc"), f"BUILD={tmp_path}", f"OUT={tmp_path}/libboa_b200.so",
+            "PYTHON=false", "BIND_CXX=no-compiler", "lib"]
+    out = subprocess.run(make, capture_output=True, text=True)
+    assert out.returncode == 0, out.stderr
+    assert "ssm.cu" in out.stdout and "libboa_b200.so" in out.stdout
+    assert "no-compiler" not in out.stdout and "ops_bind" not in out.stdout
