@@ -213,3 +213,33 @@ def test_states_of_another_depth_are_refused_gpu():
     with torch.no_grad():
         m.forward_layers(x, state)
         m.step_layers(x[:, 0], state)
+
+
+# ------------------------------------------------------------------- gradients with vector accesses throughout
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens", [None, (20, 7, 0)])
+def test_parameter_gradients_match_oracle_at_aligned_sizes(d, lens):
+    """d_model 64 and 128, whose projections' rows the scan reads and whose gradients it writes by vectors."""
+    import test_layers_gpu as base
+    from train import train_step
+    m = base._model(d, 1, seed=5) if d == 64 else _model128()
+    sd = base._leaves(m)
+    batch = _bytes(3, 21, 50)
+    n = None if lens is None else torch.tensor(lens) + torch.tensor([1, 1, 0])
+    loss = train_step(m, batch.cuda(), torch.optim.SGD(m.parameters(), lr=0.0), F.cross_entropy, lens=n)
+    logits, _ = base._reference(sd, batch[:, :-1])
+    targets = batch[:, 1:].clone()
+    if lens is not None:
+        for i, v in enumerate(lens):
+            targets[i, v:] = -100
+    want = F.cross_entropy(logits.reshape(-1, 256), targets.reshape(-1))
+    want.backward()
+    base._near(loss, want, "loss")
+    for k, p in m.named_parameters():
+        base._near(p.grad, sd[k].grad, k)
+
+
+def _model128():
+    from model import seeded_model
+    return seeded_model(128, 1, 256, 5, weight_format="bf16").cuda()
