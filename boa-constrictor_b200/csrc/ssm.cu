@@ -946,11 +946,13 @@ __global__ void __launch_bounds__(256) k_ssm_step(const boa_ssm_args a) {
 static int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 // Parts of the length for the forward call.  One where the rows alone give 256
-// blocks: at 256 blocks one part and many cost the same (203 and 202 us at 16 x
-// 2048 x 512; 54 and 67 us at 64 x 512 x 128), at 128 blocks many win (205
-// against 348 us at 8 x 4096 x 512), at 512 one does (554 against 692 us at 32 x
-// 4096 x 512).  Else enough parts for two rounds of the blocks that the SMs
-// hold, no part shorter than 64 tokens.
+// blocks; one part against many (1776 blocks), bf16: at 256 blocks 159 and 206 us
+// (16 x 2048 x 512), 45 and 71 us (64 x 512 x 128), at 512 blocks 538 and 698 us
+// (32 x 4096 x 512); at 192 blocks 307 and 292 us (12 x 4096 x 512), at 128 blocks
+// 265 and 212 us (8 x 4096 x 512), at 64 blocks 262 and 116 us (4 x 4096 x 512).
+// Else enough parts for three rounds of the four blocks that an SM holds (two
+// rounds and one and a half: 410 and 441 against 404 us at 1 x 67109 x 512, 208
+// and 222 against 212 us at 8 x 4096 x 512), no part shorter than 64 tokens.
 static SsmPlan plan_forward(const boa_ssm_args& a) {
   SsmPlan p{};
   p.cblocks = (a.channels + kCh - 1) / kCh;
@@ -978,7 +980,13 @@ static int back_groups(const boa_ssm_args& a) {
 // Parts for the backward call, whose blocks have an SM each: of 1 to 8 rounds of
 // 148 blocks, the one with the least tokens to walk one after the other (about
 // 6 tokens' time a block for its start and end), more rounds where they cost
-// at most 3 % more, since rows of different lengths then even out.
+// at most 3 % more, since rows of different lengths then even out.  The pass for
+// the parts' end gradients is not in this cost, and neither are the rows' lengths,
+// which the host does not know.  One part against the parts taken, at 512 channels
+// bf16: rows of half to full length gain (148 x 4096: 6603 and 6485 us; 128 x 4096:
+// 6499 and 5436 us), full rows enough to fill the SMs lose (128 x 4096: 6629 and
+// 7082 us; 148 x 4096: 6684 and 8037 us; 296 x 2048: 6631 and 7847 us), fewer gain
+// (64 x 4096: 6590 and 3566 us; 32 x 4096: 6537 and 1882 us).
 static SsmPlan plan_backward(const boa_ssm_args& a) {
   SsmPlan p{};
   p.cblocks = (a.channels + kCh - 1) / kCh;
