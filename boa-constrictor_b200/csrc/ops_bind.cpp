@@ -151,17 +151,20 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* fptr(const Tensor& t) { return static_cast<float*>(ptr(t)); }
 bool misaligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0; }
 
+// Memory as the values are: a view that torch marks as negated holds the other sign.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // A parameter as contiguous, 16-byte aligned fp32 (differentiable).
 Tensor param(const Tensor& t) {
   if (!t.defined()) return t;
-  Tensor r = t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
+  Tensor r = plain(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat));
   if (!r.is_contiguous()) r = r.contiguous();
   return misaligned(r) ? r.clone() : r;
 }
 // Channels contiguous; other strides stay as they are.
 Tensor rows(const Tensor& t) {
-  return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+  return plain(!t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous());
 }
+Tensor whole(const Tensor& t) { return t.defined() ? plain(t.contiguous()) : t; }
 // An input of a step apart from the state that the step changes in place: one that shares its memory would be read by
 // some threads after others have written it.
 Tensor apart(const Tensor& t, const Tensor& state) {
@@ -337,7 +340,7 @@ struct CausalConv : torch::autograd::Function<CausalConv> {
     OnDevice on(x);
     boa_conv_args a = conv_args(x, w, b, ctx->saved_data["silu"].toBool(), state, s[4]);
     const Tensor dy = upstream(up[0], x);
-    const Tensor dout = up.size() > 1 && up[1].defined() ? up[1].contiguous() : Tensor();
+    const Tensor dout = up.size() > 1 && up[1].defined() ? whole(up[1]) : Tensor();
     Tensor dx = like(x), dw = like(w), db = like(b), ds = like(state);
     a.dy = ptr(dy);
     a.dy_bs = dy.stride(0);
@@ -381,7 +384,7 @@ variable_list causal_conv(const Tensor& x_, const Tensor& weight, const Tensor& 
   reverse_mode_only(who, {&x_, &weight, &bias, &state_});
   check_device(who, x_, {&w, &bias, &state_, &lens});
   w = param(w);
-  const Tensor b = param(bias), x = rows(x_), state = state_.defined() ? state_.contiguous() : state_;
+  const Tensor b = param(bias), x = rows(x_), state = whole(state_);
   if (wants_grad({&x, &w, &b, &state})) return CausalConv::apply(x, w, opt(b), opt(state), opt(lens), silu, return_state);
   return conv_forward(x, w, b, state, lens, silu, return_state);
 }
@@ -395,7 +398,7 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   if (bias.defined()) check_shape(who, "bias", bias, {e});
   check_shape(who, "state", state, {n, w.size(1) - 1, e});
   check_same(who, "state", x_, state);
-  if (!state.is_contiguous()) refuse(text(who, ": state is updated in place and must be contiguous"));
+  if (!state.is_contiguous() || state.is_neg()) refuse(text(who, ": state is updated in place and must be contiguous"));
   no_tracing(who);
   reverse_mode_only(who, {&x_, &state, &weight, &bias});
   check_device(who, x_, {&state, &w, &bias});
@@ -491,7 +494,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
     OnDevice on(x);
     boa_ssm_args a = ssm_args(i, ctx->saved_data["softplus"].toBool());
     const Tensor dy = upstream(up[0], x);
-    const Tensor dout = up.size() > 1 && up[1].defined() ? up[1].contiguous() : Tensor();
+    const Tensor dout = up.size() > 1 && up[1].defined() ? whole(up[1]) : Tensor();
     Tensor dx = like(x), ddt = like(i.dt), dA = like(i.A), dB = like(i.B), dC = like(i.C), dD = like(i.D),
            dz = like(i.z), dbias = like(i.bias), ds = like(i.state);
     a.checkpoints = fptr(s[10]);
@@ -573,7 +576,7 @@ variable_list ssm_scan(SsmIn i, bool softplus, bool return_state) {
 Tensor ssm_step(SsmIn i, bool softplus) {
   const char* who = "ssm_step";
   ssm_check(who, i, 2);
-  if (!i.state.is_contiguous() || misaligned(i.state))
+  if (!i.state.is_contiguous() || i.state.is_neg() || misaligned(i.state))
     refuse(text(who, ": state is updated in place and must be contiguous and 16-byte aligned"));
   no_tracing(who);
   reverse_mode_only(who, {&i.x, &i.dt, &i.state, &i.A, &i.B, &i.C, &i.D, &i.z, &i.bias});

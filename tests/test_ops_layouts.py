@@ -111,3 +111,38 @@ def test_layer_norm_of_strided_rows(rows, width, edge, kind):
     m = n + rows / 8 + 64
     for name, got, v, s, k in zip(("y", "dx", "dw", "db"), (y,) + grads, vals, scales, (n, n, m, m)):
         ref.close(name, got, v, s, k)
+
+
+def test_negated_views():
+    """A view that torch marks as negated (the imaginary part of a conjugate) holds the other sign in memory."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    neg = lambda t: torch._neg_view(-t)  # noqa: E731
+    x, w, b, dy = r(6, 32), r(32), r(32), r(6, 32)
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    one = [t.detach().requires_grad_() for t in (x, w, b)]
+    two = [neg(t).detach().requires_grad_() for t in (x, w, b)]
+    for f in (lambda x, w, b: ops.layer_norm(x, w, b),
+              lambda x, w, b: ops.causal_conv(x[None], w[:, None] * torch.ones(4, device="cuda"), b),
+              lambda x, w, b: ops.ssm_scan(x[None], x[None], -torch.ones(32, 16, device="cuda"), x[None, :, :16],
+                                           x[None, :, 16:], w, x[None], b)):
+        y, z = f(*one), f(*two)
+        assert torch.equal(y, z)
+        up = dy.view(y.shape)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, one, up), torch.autograd.grad(z, two, neg(up))))
+    A, h, window, k = -torch.ones(32, 16, device="cuda"), r(6, 32, 16), r(6, 3, 32), r(32, 4)
+    for f in (neg, lambda t: t):
+        y, end = ops.ssm_scan(x[None], x[None], f(A), f(x[None, :, :16]), f(x[None, :, 16:]), state=f(h[:1]), return_state=True)
+        u, win = ops.causal_conv(x[None], f(k), state=f(window[:1]), return_state=True)
+        s, t = h.clone(), window.clone()
+        v = ops.ssm_step(f(x), f(x), s, f(A), f(x[:, :16]), f(x[:, 16:]))
+        q = ops.causal_conv_step(f(x), t, f(k))
+        now = (y, end, u, win, s, t, v, q)
+        if f is neg:
+            first = now
+    assert all(torch.equal(p, q) for p, q in zip(first, now))
+    with pytest.raises(ValueError, match="in place"):
+        ops.ssm_step(x, x, neg(h), A, x[:, :16], x[:, 16:])
+    with pytest.raises(ValueError, match="in place"):
+        ops.causal_conv_step(x, neg(window), k)
