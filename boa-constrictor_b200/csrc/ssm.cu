@@ -391,7 +391,8 @@ static __global__ void __launch_bounds__(128) k_ssm_join(int64_t n, int E, int p
     for (int j = 0; j < kAhead; ++j)
       if (k0 + j < parts) {
         ends[(s + j * step) * en + r] = carry;
-        carry = fmaf(ex2(A2 * sum[j]), carry, own[j]);
+        // nothing comes in: nothing is passed on, also where a decay above 1 has overflowed over the part
+        carry = carry == 0.0f ? own[j] : fmaf(ex2(A2 * sum[j]), carry, own[j]);
       }
     s += kAhead * step;
   }

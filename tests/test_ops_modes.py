@@ -111,3 +111,25 @@ def test_scan_channels_that_forget_at_once():
     with torch.no_grad():
         one = ops.ssm_step(x[:, 0].cuda(), torch.full((nb, e), -200.0).cuda(), st, A.cuda(), B[:, 0].cuda(), C[:, 0].cuda())
     assert torch.equal(st, state.cuda()) and torch.isfinite(one).all()      # d underflows to 0: nothing moves
+
+
+@pytest.mark.gpu
+def test_scan_split_over_states_that_grow():
+    """A above 0: a part's decay overflows fp32 (e^3 a token) while the state that enters it is still 0, which is then
+    0 behind it too.  Only the last 16 tokens of a row have an input, so no value of the definition leaves fp32."""
+    import ops_reference as ref
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    length, e = 1200, 8
+    x, dt = r(2, length, e), 3.0 + 0.1 * r(2, length, e)
+    lens = torch.tensor([length, 700], dtype=torch.int32)
+    for i, n in enumerate(lens.tolist()):
+        x[i, :n - 16] = 0.0
+    B, C, A = r(2, length, 16), r(2, length, 16), torch.ones(e, 16)
+    want = ref.scan(*[t.double() for t in (x, dt, A, B, C)], None, None, None, True, None, lens, torch.zeros_like(x).double(),
+                    None)
+    with torch.no_grad():
+        y, h = ops.ssm_scan(*[t.cuda() for t in (x, dt, A, B, C)], lens=lens.cuda(), return_state=True)
+    # 16 tokens, each with an exponent of up to 4.7 whose 3 roundings the decay scales by 3.3, and 5 more; and 96 at the end
+    ref.close("y", y, *want["y"], 16 * 15 + 96)
+    ref.close("state", h, *want["state"], 16 * 15 + 64)
