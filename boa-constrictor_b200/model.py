@@ -85,9 +85,12 @@ class Mamba(nn.Module):
         self.out_proj = nn.Linear(E, d_model, bias=False)
 
     def init_state(self, batch_size: int, device=None, dtype=None):
-        """(convolution window [B, 3, E], scan state [B, E, 16] fp32) before the first token."""
+        """(convolution window [B, 3, E], scan state [B, E, 16] fp32) before the first token.  The window has
+        the type of the activations: the weights' one, or that of the autocast region."""
         w = self.in_proj.weight
-        device, dtype = device or w.device, dtype or w.dtype
+        device = torch.device(device) if device else w.device
+        if dtype is None:
+            dtype = torch.get_autocast_dtype(device.type) if torch.is_autocast_enabled(device.type) else w.dtype
         return (torch.zeros(batch_size, D_CONV - 1, self.d_inner, dtype=dtype, device=device),
                 torch.zeros(batch_size, self.d_inner, D_STATE, dtype=torch.float32, device=device))
 

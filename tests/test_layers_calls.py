@@ -243,3 +243,26 @@ def test_parameter_gradients_match_oracle_at_aligned_sizes(d, lens):
 def _model128():
     from model import seeded_model
     return seeded_model(128, 1, 256, 5, weight_format="bf16").cuda()
+
+
+# ------------------------------------------------------------------- steps under autocast
+def test_first_state_has_the_type_of_the_region():
+    m = _model(64, 1)
+    kinds = lambda s: [t.dtype for t in s[0]]  # noqa: E731
+    with torch.autocast("cpu", torch.bfloat16):
+        assert kinds(m.init_layers(2)) == [torch.bfloat16, torch.float32]
+        assert kinds(m.init_layers(2, torch.float16)) == [torch.float16, torch.float32]
+    assert kinds(m.init_layers(2)) == [torch.float32, torch.float32]
+
+
+@pytest.mark.gpu
+def test_steps_under_autocast():
+    """Single tokens from the first state, in bf16, against the prompt: one sequence.  A layer's 2^-9 roundings of
+    bf16 values differ where fp32 values lie on the other side of one: about 10 of them a logit, in the 2-norm."""
+    m = _model(64, 1).cuda()
+    x = _bytes(3, 12, 60).cuda()
+    with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+        whole = m.forward_layers(x).float()
+        state = m.init_layers(3)
+        steps = torch.stack([m.step_layers(x[:, t], state) for t in range(12)], 1).float()
+    assert (whole - steps).norm() <= 10 * 2.0 ** -9 * whole.norm()
